@@ -26,7 +26,8 @@ EXPORTS = ("flashmhf_abi_version", "flashmhf_forward_workspace_bytes", "flashmhf
            "flashmhf_selftest_bounded_wait", "flashmhf_prologue_forward_dtype", "flashmhf_prologue_backward_dtype",
            "flashmhf_lm_rmsnorm_forward_dtype", "flashmhf_lm_rmsnorm_backward_dtype", "flashmhf_lm_rope_pair",
            "flashmhf_lm_add_rmsnorm_forward", "flashmhf_lm_add_rmsnorm_backward",
-           "flashmhf_backward_plan")
+           "flashmhf_backward_plan", "flashmhf_paged_append", "flashmhf_paged_attention_workspace_bytes", "flashmhf_paged_attention",
+           "flashmhf_prompt_attention")
 
 
 class Tensor(C.Structure):
@@ -71,6 +72,35 @@ class PrologueBwdParams(C.Structure):
     _fields_ = [("fwd", PrologueParams), ("dQ", C.c_void_p), ("dq_stride", C.c_int64 * 3), ("dR", C.c_void_p),
                 ("dX", C.c_void_p), ("d_router", C.c_void_p), ("d_norm_weight", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class KVPagesParams(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("page_stride", C.c_int64),
+                ("num_pages", C.c_int32), ("n_kv", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class KVSequences(C.Structure):
+    _fields_ = [("lengths", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64), ("B", C.c_int32), ("max_pages", C.c_int32)]
+
+
+class PagedAppendParams(C.Structure):
+    _fields_ = [("pages", KVPagesParams), ("seq", KVSequences), ("cu_seqlens", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+                ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("cos_t", C.c_void_p), ("sin_t", C.c_void_p),
+                ("tokens", C.c_int32), ("n_q", C.c_int32), ("max_positions", C.c_int32)]
+
+
+class PagedAttentionParams(C.Structure):
+    _fields_ = [("pages", KVPagesParams), ("seq", KVSequences), ("q", C.c_void_p), ("o", C.c_void_p), ("q_stride", C.c_int64 * 3),
+                ("o_stride", C.c_int64 * 3), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("n_q", C.c_int32), ("n_new", C.c_int32), ("scale", C.c_float)]
+
+
+class PromptAttentionParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("q_stride", C.c_int64 * 2),
+                ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("o_stride", C.c_int64 * 2), ("lse", C.c_void_p),
+                ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("B", C.c_int32), ("tokens_q", C.c_int32), ("tokens_k", C.c_int32),
+                ("n_q", C.c_int32), ("n_kv", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float)]
 
 
 class FlashMHFError(RuntimeError):
@@ -133,6 +163,14 @@ def load():
         lib.flashmhf_lm_rmsnorm_backward.restype = C.c_int
         lib.flashmhf_lm_rmsnorm_backward.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                      C.c_size_t, C.c_int64, C.c_int32, C.c_float, C.c_void_p]
+        lib.flashmhf_paged_append.restype = C.c_int
+        lib.flashmhf_paged_append.argtypes = [C.POINTER(PagedAppendParams), C.c_void_p]
+        lib.flashmhf_paged_attention_workspace_bytes.restype = C.c_size_t
+        lib.flashmhf_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionParams)]
+        lib.flashmhf_paged_attention.restype = C.c_int
+        lib.flashmhf_paged_attention.argtypes = [C.POINTER(PagedAttentionParams), C.c_void_p]
+        lib.flashmhf_prompt_attention.restype = C.c_int
+        lib.flashmhf_prompt_attention.argtypes = [C.POINTER(PromptAttentionParams), C.c_void_p]
         lib.flashmhf_selftest_bounded_wait.restype = C.c_int
         lib.flashmhf_selftest_bounded_wait.argtypes = [C.c_longlong, C.c_void_p]
         lib.flashmhf_device_status.restype = C.c_int
@@ -180,9 +218,11 @@ def check(status):
 
 
 def device_status():
-    """Synchronise the current device and raise if a kernel gave up on a bounded wait since the last call.
+    """Synchronise the current device and raise if a kernel gave up on a bounded wait since the last call, or if a serving
+    kernel met a page number, length or position out of range.
 
-    The launch whose wait ran out left its outputs unwritten; later launches ran normally.  Reading clears the word."""
+    The launch whose wait ran out left its outputs unwritten, and what was out of range was left out; later launches ran
+    normally.  Reading clears the word."""
     code = C.c_int(0)
     st = load().flashmhf_device_status(C.byref(code))
     if st != 0:

@@ -145,6 +145,7 @@ const char *flashmhf_strerror(int status) {
         case FLASHMHF_ERR_DEVICE_TIMEOUT: return "a kernel gave up on a bounded wait";
         case FLASHMHF_ERR_SCRATCH_LIMIT:
             return "these dims need more scratch than the library's built-in 72 MiB array; use flashmhf_backward with a workspace";
+        case FLASHMHF_ERR_DEVICE_INDEX: return "a serving kernel met a page number, length or position out of range and left it out";
         default: return "unknown status";
     }
 }
@@ -422,6 +423,100 @@ int flashmhf_lm_add_rmsnorm_backward(const void *sum, const void *w, int32_t w_d
     return rc;
 }
 
+// bf16 rows of the serving calls: innermost dimension contiguous, everything else in steps of 16 bytes.
+static int check_rows(const void *p, const int64_t *stride, int n) {
+    if (!p) return FLASHMHF_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(p) & 15u) return FLASHMHF_ERR_MISALIGNED;
+    for (int i = 0; i < n; ++i)
+        if (stride[i] < 0 || stride[i] % 8 != 0) return FLASHMHF_ERR_BAD_STRIDE;
+    return FLASHMHF_OK;
+}
+static int check_pages(const flashmhf_kv_pages &g, const flashmhf_kv_sequences &s) {
+    if (g.head_dim != 64 && g.head_dim != 96 && g.head_dim != 128) return FLASHMHF_ERR_BAD_SHAPE;
+    if (g.page_size != 16 && g.page_size != 32 && g.page_size != 64 && g.page_size != 128) return FLASHMHF_ERR_BAD_SHAPE;
+    if (g.num_pages < 1 || g.n_kv < 1 || g.n_kv > 65535 || s.B < 1 || s.max_pages < 1) return FLASHMHF_ERR_BAD_SHAPE;
+    if ((long long)s.max_pages * g.page_size > 0x7fffffffll) return FLASHMHF_ERR_BAD_SHAPE;   // positions are 32-bit numbers
+    if (!g.k || !g.v || !g.k_scale || !g.v_scale || !s.lengths || !s.table) return FLASHMHF_ERR_NULL;
+    if ((reinterpret_cast<uintptr_t>(g.k) | reinterpret_cast<uintptr_t>(g.v)) & 15u) return FLASHMHF_ERR_MISALIGNED;
+    if ((reinterpret_cast<uintptr_t>(g.k_scale) | reinterpret_cast<uintptr_t>(g.v_scale) | reinterpret_cast<uintptr_t>(s.lengths) |
+         reinterpret_cast<uintptr_t>(s.table)) & 3u)
+        return FLASHMHF_ERR_MISALIGNED;
+    if (g.page_stride % 16 != 0 || g.page_stride < (int64_t)g.n_kv * g.page_size * g.head_dim || s.table_stride < s.max_pages)
+        return FLASHMHF_ERR_BAD_STRIDE;
+    return FLASHMHF_OK;
+}
+
+int flashmhf_paged_append(const flashmhf_paged_append_params *p, void *stream) {
+    if (!p) return FLASHMHF_ERR_NULL;
+    int rc = check_pages(p->pages, p->seq);
+    if (rc) return rc;
+    if (p->tokens < 1 || p->max_positions < 1 || (p->q && (p->n_q < 1 || p->n_q > 65535))) return FLASHMHF_ERR_BAD_SHAPE;
+    if (!p->cu_seqlens && p->tokens != p->seq.B) return FLASHMHF_ERR_BAD_SHAPE;
+    if ((rc = check_rows(p->k, p->k_stride, 2)) != 0 || (rc = check_rows(p->v, p->v_stride, 2)) != 0) return rc;
+    if (p->q && ((rc = check_rows(p->q, p->q_stride, 2)) != 0 || (rc = check_rows(p->q_out, p->q_stride, 0)) != 0)) return rc;
+    if (!p->cos_t || !p->sin_t) return FLASHMHF_ERR_NULL;
+    if (((reinterpret_cast<uintptr_t>(p->cos_t) | reinterpret_cast<uintptr_t>(p->sin_t) | reinterpret_cast<uintptr_t>(p->k_out)) & 15u) ||
+        (reinterpret_cast<uintptr_t>(p->cu_seqlens) & 3u))
+        return FLASHMHF_ERR_MISALIGNED;
+    if ((rc = check_arch()) != 0) return rc;
+    const DeviceCtl *ctl = device_ctl();
+    if (!ctl) return FLASHMHF_ERR_CUDA;
+    int n = 0;
+    rc = paged_append(*p, *ctl, static_cast<cudaStream_t>(stream), &n);
+    g_launches += (uint64_t)n;
+    return rc;
+}
+
+static int check_paged_attention(const flashmhf_paged_attention_params *p) {
+    if (!p) return FLASHMHF_ERR_NULL;
+    int rc = check_pages(p->pages, p->seq);
+    if (rc) return rc;
+    if (p->n_q < 1 || p->n_q > 65535 || p->n_q % p->pages.n_kv != 0 || p->n_new < 1 || p->n_new > 16 || !(p->scale - p->scale == 0.f))
+        return FLASHMHF_ERR_BAD_SHAPE;
+    if ((rc = check_rows(p->q, p->q_stride, 3)) != 0 || (rc = check_rows(p->o, p->o_stride, 3)) != 0) return rc;
+    return reinterpret_cast<uintptr_t>(p->lse) & 3u ? FLASHMHF_ERR_MISALIGNED : FLASHMHF_OK;
+}
+
+size_t flashmhf_paged_attention_workspace_bytes(const flashmhf_paged_attention_params *p) {
+    return check_paged_attention(p) == FLASHMHF_OK ? paged_attention_workspace_bytes(*p) : 0;
+}
+
+int flashmhf_paged_attention(const flashmhf_paged_attention_params *p, void *stream) {
+    int rc = check_paged_attention(p);
+    if (rc) return rc;
+    const size_t need = paged_attention_workspace_bytes(*p);
+    if (need && (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255u))) return FLASHMHF_ERR_WORKSPACE;
+    if ((rc = check_arch()) != 0) return rc;
+    const DeviceCtl *ctl = device_ctl();
+    if (!ctl) return FLASHMHF_ERR_CUDA;
+    int n = 0;
+    rc = paged_attention(*p, *ctl, static_cast<cudaStream_t>(stream), &n);
+    g_launches += (uint64_t)n;
+    return rc;
+}
+
+int flashmhf_prompt_attention(const flashmhf_prompt_attention_params *p, void *stream) {
+    if (!p) return FLASHMHF_ERR_NULL;
+    if (p->head_dim != 64 && p->head_dim != 96 && p->head_dim != 128) return FLASHMHF_ERR_BAD_SHAPE;
+    if (p->B < 1 || p->tokens_q < 1 || p->tokens_k < 0 || p->n_kv < 1 || p->n_q < 1 || p->n_q > 65535 || p->n_q % p->n_kv != 0 ||
+        !(p->scale - p->scale == 0.f))
+        return FLASHMHF_ERR_BAD_SHAPE;
+    int rc = FLASHMHF_OK;
+    if ((rc = check_rows(p->q, p->q_stride, 2)) != 0 || (rc = check_rows(p->k, p->k_stride, 2)) != 0 || (rc = check_rows(p->v, p->v_stride, 2)) != 0 ||
+        (rc = check_rows(p->o, p->o_stride, 2)) != 0)
+        return rc;
+    if (!p->cu_q || !p->cu_k) return FLASHMHF_ERR_NULL;
+    if ((reinterpret_cast<uintptr_t>(p->cu_q) | reinterpret_cast<uintptr_t>(p->cu_k) | reinterpret_cast<uintptr_t>(p->lse)) & 3u)
+        return FLASHMHF_ERR_MISALIGNED;
+    if ((rc = check_arch()) != 0) return rc;
+    const DeviceCtl *ctl = device_ctl();
+    if (!ctl) return FLASHMHF_ERR_CUDA;
+    int n = 0;
+    rc = prompt_attention(*p, *ctl, static_cast<cudaStream_t>(stream), &n);
+    g_launches += (uint64_t)n;
+    return rc;
+}
+
 int flashmhf_profile_begin(int max_marks) {
     std::lock_guard<std::mutex> lk(g_mu);
     if (g_prof.on || max_marks < 2) return FLASHMHF_ERR_BAD_SHAPE;
@@ -482,6 +577,7 @@ int flashmhf_device_status(int *code) {
         return FLASHMHF_ERR_CUDA;
     }
     if (code) *code = v;
+    if (v >= kFirstIndexCode && v <= kLastIndexCode) return FLASHMHF_ERR_DEVICE_INDEX;
     return v == 0 ? FLASHMHF_OK : FLASHMHF_ERR_DEVICE_TIMEOUT;
 }
 

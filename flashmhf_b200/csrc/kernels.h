@@ -76,6 +76,14 @@ size_t lm_rmsnorm_backward_workspace_bytes(long long rows, int n);
 int lm_rmsnorm_backward(const void *x, const void *w, bool bf16_w, const void *g, const void *gh, void *dx, void *dw, void *workspace,
                         size_t workspace_bytes, long long rows, int n, float eps, cudaStream_t st, int *n_launch);
 
+// ---- serving: paged 8-bit key/value cache and attention over packed prompts (arguments checked by api.cu) ----
+int paged_append(const flashmhf_paged_append_params &p, const DeviceCtl &ctl, cudaStream_t st, int *n_launch);
+size_t paged_attention_workspace_bytes(const flashmhf_paged_attention_params &p);
+int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &ctl, cudaStream_t st, int *n_launch);
+int prompt_attention(const flashmhf_prompt_attention_params &p, const DeviceCtl &ctl, cudaStream_t st, int *n_launch);
+// Status-word codes in this range name an index out of range, not a wait that ran out.
+constexpr int kFirstIndexCode = 400, kLastIndexCode = 599;
+
 // Launch.  `early`: with programmatic stream serialization, so that the kernel may start before the one ahead of it on the
 // stream has ended (as soon as that one's CTAs have all asked for it, or exited).
 // `cluster`: CTAs (along x) of a thread-block cluster.

@@ -45,6 +45,10 @@ struct Api {
     decltype(&flashmhf_lm_rope_pair) lm_rope_pair = nullptr;
     decltype(&flashmhf_lm_add_rmsnorm_forward) add_rmsnorm_forward = nullptr;
     decltype(&flashmhf_lm_add_rmsnorm_backward) add_rmsnorm_backward = nullptr;
+    decltype(&flashmhf_paged_append) paged_append = nullptr;
+    decltype(&flashmhf_paged_attention_workspace_bytes) paged_attention_ws = nullptr;
+    decltype(&flashmhf_paged_attention) paged_attention = nullptr;
+    decltype(&flashmhf_prompt_attention) prompt_attention = nullptr;
     PyObject *error_type = nullptr;  // flashmhf_b200._lib.FlashMHFError(status, message)
 };
 Api api;
@@ -75,6 +79,10 @@ void bind(uintptr_t handle, py::object error_type) {
     get(api.lm_rope_pair, "flashmhf_lm_rope_pair");
     get(api.add_rmsnorm_forward, "flashmhf_lm_add_rmsnorm_forward");
     get(api.add_rmsnorm_backward, "flashmhf_lm_add_rmsnorm_backward");
+    get(api.paged_append, "flashmhf_paged_append");
+    get(api.paged_attention_ws, "flashmhf_paged_attention_workspace_bytes");
+    get(api.paged_attention, "flashmhf_paged_attention");
+    get(api.prompt_attention, "flashmhf_prompt_attention");
     Py_XDECREF(api.error_type);
     api.error_type = error_type.release().ptr();
 }
@@ -778,6 +786,237 @@ std::pair<Tensor, Tensor> add_rmsnorm(const Tensor &h, const Tensor &d, const Te
     return {o[0], o[1]};
 }
 
+// ------------------------------------------------------------------------------------------------ serving
+// Shapes and types are looked at first, then devices; the kernels take addresses and trust what passed here.
+void no_gradients(const char *who, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts) {
+        if (!t->defined()) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t->requires_grad()) && !has_tangent(*t), who,
+                                    " has no derivative: call it under torch.no_grad(), or on tensors that do not require gradients");
+    }
+}
+void same_device(const char *who, const Tensor &first, std::initializer_list<const Tensor *> ts) {
+    bool ok = first.is_cuda();
+    for (const Tensor *t : ts) ok = ok && (!t->defined() || t->device() == first.device());
+    if (!ok) throw py::value_error(std::string(who) + " runs on CUDA tensors of one device; there is no CPU path");
+}
+void bf16_heads(const char *name, const Tensor &t, int64_t heads, int64_t hd) {
+    if (t.dim() != 3 || (heads > 0 && t.size(1) != heads) || t.size(2) != hd)
+        throw py::value_error(std::string(name) + " must be [tokens, " + (heads > 0 ? std::to_string(heads) : "heads") + ", " + std::to_string(hd) +
+                              "], got " + dims_text(t));
+    if (t.scalar_type() != at::kBFloat16) throw py::type_error(std::string(name) + " must be torch.bfloat16, got " + c10::toString(t.scalar_type()));
+}
+Tensor int_row(const char *name, const Tensor &t, int64_t n) {
+    if (t.dim() != 1 || t.size(0) != n) throw py::value_error(std::string(name) + " must have " + std::to_string(n) + " entries, got " + dims_text(t));
+    if (t.scalar_type() != at::kInt) throw py::type_error(std::string(name) + " must be torch.int32, got " + c10::toString(t.scalar_type()));
+    return t.contiguous();
+}
+int64_t sequences(const char *name, const Tensor &cu) {
+    if (cu.dim() != 1 || cu.size(0) < 1) throw py::value_error(std::string(name) + " must be [sequences + 1], got " + dims_text(cu));
+    return cu.size(0) - 1;
+}
+// bf16 rows that the kernels read in place (unit inner stride, everything else in 16-byte steps); else a copy.
+bool rows_ok(const Tensor &t) {
+    const int64_t n = t.dim();
+    if (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) return false;
+    if (t.stride(n - 1) != 1) return false;
+    for (int64_t i = 0; i + 1 < n; ++i)
+        if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
+    return true;
+}
+Tensor rows(const Tensor &t) { return rows_ok(t) ? t : t.contiguous(); }
+void strides_of(const Tensor &t, int64_t *to) {   // of all but the innermost dimension; one of extent 1 has none that matters
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) to[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+Tensor given_or_new(const std::optional<Tensor> &out, const Tensor &like) {
+    if (!out) return at::empty(like.sizes(), like.options());
+    if (out->sizes() != like.sizes() || out->scalar_type() != like.scalar_type() || out->device() != like.device() || !rows_ok(*out))
+        throw py::value_error("out must be like q, its last dimension contiguous and the others in steps of 16 bytes");
+    TORCH_CHECK_NOT_IMPLEMENTED(!out->requires_grad(), "out must not require gradients");
+    return *out;
+}
+float softmax_scale(const std::optional<double> &scale, int64_t hd) {
+    const double s = scale ? *scale : 1.0 / std::sqrt((double)hd);
+    if (!std::isfinite(s)) throw py::value_error("scale must be finite");
+    return (float)s;
+}
+
+flashmhf_kv_pages pages_of(const Tensor &k, const Tensor &v, const Tensor &ks, const Tensor &vs) {
+    if (k.dim() != 4 || v.sizes() != k.sizes()) throw py::value_error("pages must be [num_pages, n_kv, page_size, head_dim] twice, got " + dims_text(k) + " and " + dims_text(v));
+    const int64_t n = k.size(0), h = k.size(1), P = k.size(2), hd = k.size(3);
+    if (hd != 64 && hd != 96 && hd != 128) throw py::value_error("head_dim " + std::to_string(hd) + " not supported (64, 96 or 128)");
+    if (P != 16 && P != 32 && P != 64 && P != 128) throw py::value_error("page_size " + std::to_string(P) + " not supported (16, 32, 64 or 128)");
+    if (n < 1 || h < 1 || h > 65535 || n > INT32_MAX) throw py::value_error("pages must have at least one page and one head, got " + dims_text(k));
+    for (const Tensor *t : {&k, &v}) {
+        if (t->scalar_type() != at::kFloat8_e4m3fn) throw py::type_error(std::string("pages must be torch.float8_e4m3fn, got ") + c10::toString(t->scalar_type()));
+        if (t->stride(3) != 1 || t->stride(2) != hd || (h > 1 && t->stride(1) != P * hd) || (n > 1 && (t->stride(0) % 16 != 0 || t->stride(0) < h * P * hd)) ||
+            (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15u))
+            throw py::value_error("a page must be contiguous, and pages must be 16-byte aligned and not overlap");
+    }
+    if (n > 1 && k.stride(0) != v.stride(0)) throw py::value_error("k and v must have the same distance between pages");
+    for (const Tensor *t : {&ks, &vs}) {
+        if (t->scalar_type() != at::kFloat) throw py::type_error(std::string("scales must be torch.float32, got ") + c10::toString(t->scalar_type()));
+        if (t->dim() != 2 || t->size(0) != n || t->size(1) != h || !t->is_contiguous())
+            throw py::value_error("scales must be contiguous [" + std::to_string(n) + ", " + std::to_string(h) + "], got " + dims_text(*t));
+    }
+    flashmhf_kv_pages g{};
+    g.k = k.data_ptr(); g.v = v.data_ptr();
+    g.k_scale = static_cast<float *>(ks.data_ptr()); g.v_scale = static_cast<float *>(vs.data_ptr());
+    g.page_stride = n > 1 ? k.stride(0) : h * P * hd;
+    g.num_pages = (int32_t)n; g.n_kv = (int32_t)h; g.page_size = (int32_t)P; g.head_dim = (int32_t)hd;
+    return g;
+}
+Tensor table_rows(const Tensor &table, int64_t B, int64_t P) {
+    if (table.dim() != 2 || table.size(0) != B || table.size(1) < 1)
+        throw py::value_error("page_table must be [" + std::to_string(B) + ", pages], got " + dims_text(table));
+    if (table.scalar_type() != at::kInt) throw py::type_error(std::string("page_table must be torch.int32, got ") + c10::toString(table.scalar_type()));
+    if (table.size(1) > INT32_MAX / P) throw py::value_error("page_table has room for more than 2^31 positions a sequence");
+    return table.stride(1) == 1 && (B == 1 || table.stride(0) >= table.size(1)) ? table : table.contiguous();
+}
+flashmhf_kv_sequences sequences_of(const Tensor &lengths, const Tensor &table) {
+    return flashmhf_kv_sequences{lengths.const_data_ptr<int32_t>(), table.const_data_ptr<int32_t>(), table.size(0) > 1 ? table.stride(0) : table.size(1),
+                                 (int32_t)table.size(0), (int32_t)table.size(1)};
+}
+
+std::pair<std::optional<Tensor>, std::optional<Tensor>> paged_append(const Tensor &kp, const Tensor &vp, const Tensor &ks, const Tensor &vs, const Tensor &k0,
+                                                                     const Tensor &v0, const Tensor &cos_t, const Tensor &sin_t, const Tensor &lengths0,
+                                                                     const Tensor &table0, const std::optional<Tensor> &q0,
+                                                                     const std::optional<Tensor> &cu0, bool rotated_keys) {
+    flashmhf_paged_append_params p{};
+    p.pages = pages_of(kp, vp, ks, vs);
+    const int64_t hd = p.pages.head_dim, n_kv = p.pages.n_kv, T = k0.dim() ? k0.size(0) : 0;
+    bf16_heads("k", k0, n_kv, hd);
+    bf16_heads("v", v0, n_kv, hd);
+    if (q0) bf16_heads("q", *q0, 0, hd);
+    if (v0.size(0) != T || (q0 && q0->size(0) != T)) throw py::value_error("q, k and v must have the same number of tokens");
+    if (q0 && (q0->size(1) < 1 || q0->size(1) > 65535)) throw py::value_error("q must have 1 to 65535 heads, got " + dims_text(*q0));
+    const int64_t B = cu0 ? sequences("cu_seqlens", *cu0) : T;
+    const Tensor lengths = int_row("lengths", lengths0, B), cu = cu0 ? int_row("cu_seqlens", *cu0, B + 1) : Tensor();
+    const Tensor table = B ? table_rows(table0, B, p.pages.page_size) : table0;
+    for (const Tensor *t : {&cos_t, &sin_t})
+        if (t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(1) * 2 != hd || t->size(0) < 1 || t->sizes() != cos_t.sizes() || !t->is_contiguous() ||
+            (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15u))
+            throw py::value_error("cos and sin must be contiguous fp32 [positions, " + std::to_string(hd / 2) + "]");
+    const Tensor none, &q1 = q0 ? *q0 : none;
+    same_device("paged_append", kp, {&vp, &ks, &vs, &k0, &v0, &cos_t, &sin_t, &lengths, &table0, &q1, &cu});
+    no_gradients("paged_append", {&k0, &v0, &cos_t, &sin_t, &q1, &ks, &vs});
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(kp.device());
+    const Tensor k = rows(k0), v = rows(v0), q = q0 ? rows(*q0) : Tensor();
+    std::optional<Tensor> q_out, k_out;
+    if (q0) q_out = at::empty(q.sizes(), q.options());
+    if (rotated_keys) k_out = at::empty(k.sizes(), k.options());
+    if (T == 0 || B == 0) return {q_out, k_out};
+    if (T > INT32_MAX) throw py::value_error("more than 2^31 tokens in a call");
+    p.seq = sequences_of(lengths, table);
+    p.cu_seqlens = cu0 ? cu.const_data_ptr<int32_t>() : nullptr;
+    p.k = k.data_ptr(); p.v = v.data_ptr();
+    strides_of(k, p.k_stride);
+    strides_of(v, p.v_stride);
+    if (q0) {
+        p.q = q.data_ptr();
+        p.q_out = q_out->data_ptr();
+        p.n_q = (int32_t)q.size(1);
+        strides_of(q, p.q_stride);
+    }
+    if (k_out) p.k_out = k_out->data_ptr();
+    p.cos_t = cos_t.const_data_ptr<float>(); p.sin_t = sin_t.const_data_ptr<float>();
+    p.tokens = (int32_t)T;
+    p.max_positions = (int32_t)std::min<int64_t>(cos_t.size(0), INT32_MAX);
+    check(api.paged_append(&p, current_stream(kp)));
+    return {q_out, k_out};
+}
+
+using Attended = std::pair<Tensor, std::optional<Tensor>>;
+Attended with_lse(const Tensor &o, const Tensor &lse) { return {o, lse.defined() ? std::optional<Tensor>(lse) : std::nullopt}; }
+
+Attended paged_attention(const Tensor &q0, const Tensor &kp, const Tensor &vp, const Tensor &ks, const Tensor &vs, const Tensor &lengths0,
+                           const Tensor &table0, const std::optional<double> &scale, const std::optional<Tensor> &out, bool want_lse) {
+    flashmhf_paged_attention_params p{};
+    p.pages = pages_of(kp, vp, ks, vs);
+    const int64_t hd = p.pages.head_dim, n_kv = p.pages.n_kv, dim = q0.dim();
+    if ((dim != 3 && dim != 4) || q0.size(dim - 1) != hd)
+        throw py::value_error("q must be [B, heads, " + std::to_string(hd) + "] or [B, new tokens, heads, " + std::to_string(hd) + "], got " + dims_text(q0));
+    if (q0.scalar_type() != at::kBFloat16) throw py::type_error(std::string("q must be torch.bfloat16, got ") + c10::toString(q0.scalar_type()));
+    const int64_t B = q0.size(0), n_new = dim == 4 ? q0.size(1) : 1, n_q = q0.size(dim - 2);
+    if (n_new < 1 || n_new > 16) throw py::value_error("1 to 16 new tokens a sequence, got " + std::to_string(n_new));
+    if (n_q < 1 || n_q > 65535 || n_q % n_kv != 0)
+        throw py::value_error("query heads " + std::to_string(n_q) + " must be a multiple of the pages' " + std::to_string(n_kv) + " heads");
+    const Tensor lengths = int_row("lengths", lengths0, B);
+    const Tensor table = B ? table_rows(table0, B, p.pages.page_size) : table0;
+    p.scale = softmax_scale(scale, hd);
+    same_device("paged_attention", q0, {&kp, &vp, &ks, &vs, &lengths, &table0});
+    no_gradients("paged_attention", {&q0, &ks, &vs});
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(q0.device());
+    const Tensor q = rows(q0);
+    const Tensor o = given_or_new(out, q0), lse = want_lse ? at::empty(q0.sizes().slice(0, dim - 1), q0.options().dtype(at::kFloat)) : Tensor();
+    if (B == 0) return with_lse(o, lse);
+    p.seq = sequences_of(lengths, table);
+    p.q = q.data_ptr(); p.o = o.data_ptr();
+    if (dim == 4) {
+        strides_of(q, p.q_stride);
+        strides_of(o, p.o_stride);
+    } else {
+        int64_t s[2];
+        strides_of(q, s);
+        p.q_stride[0] = s[0]; p.q_stride[2] = s[1];
+        strides_of(o, s);
+        p.o_stride[0] = s[0]; p.o_stride[2] = s[1];
+    }
+    p.lse = want_lse ? static_cast<float *>(lse.data_ptr()) : nullptr;
+    p.n_q = (int32_t)n_q; p.n_new = (int32_t)n_new;
+    p.workspace_bytes = api.paged_attention_ws(&p);
+    Tensor ws;
+    if (p.workspace_bytes) {
+        ws = scratch(std::nullopt, p.workspace_bytes, q0);
+        p.workspace = ws.data_ptr();
+    }
+    check(api.paged_attention(&p, current_stream(q0)));
+    return with_lse(o, lse);
+}
+
+Attended prompt_attention(const Tensor &q0, const Tensor &k0, const Tensor &v0, const Tensor &cu_q0, const std::optional<Tensor> &cu_k0, bool causal,
+                            const std::optional<double> &scale, const std::optional<Tensor> &out, bool want_lse) {
+    const int64_t hd = q0.dim() ? q0.size(q0.dim() - 1) : 0;
+    if (hd != 64 && hd != 96 && hd != 128) throw py::value_error("head_dim " + std::to_string(hd) + " not supported (64, 96 or 128)");
+    bf16_heads("q", q0, 0, hd);
+    bf16_heads("k", k0, 0, hd);
+    bf16_heads("v", v0, 0, hd);
+    const int64_t T = q0.size(0), Tk = k0.size(0), n_q = q0.size(1), n_kv = k0.size(1);
+    if (v0.sizes() != k0.sizes()) throw py::value_error("k and v must have the same shape, got " + dims_text(k0) + " and " + dims_text(v0));
+    if (n_kv < 1 || n_q < 1 || n_q > 65535 || n_q % n_kv != 0)
+        throw py::value_error("query heads " + std::to_string(n_q) + " must be a multiple of the " + std::to_string(n_kv) + " key/value heads");
+    const int64_t B = sequences("cu_seqlens", cu_q0);
+    const Tensor cu_q = int_row("cu_seqlens", cu_q0, B + 1), cu_k = cu_k0 ? int_row("cu_seqlens_k", *cu_k0, B + 1) : cu_q;
+    if (!cu_k0 && Tk != T) throw py::value_error("k must have as many tokens as q where cu_seqlens_k is not given");
+    flashmhf_prompt_attention_params p{};
+    p.scale = softmax_scale(scale, hd);
+    same_device("prompt_attention", q0, {&k0, &v0, &cu_q, &cu_k});
+    no_gradients("prompt_attention", {&q0, &k0, &v0});
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(q0.device());
+    const Tensor q = rows(q0), k = rows(k0), v = rows(v0);
+    const Tensor o = given_or_new(out, q0), lse = want_lse ? at::empty({T, n_q}, q0.options().dtype(at::kFloat)) : Tensor();
+    if (T == 0 || B == 0) return with_lse(o, lse);
+    if (T > INT32_MAX || Tk > INT32_MAX) throw py::value_error("more than 2^31 tokens in a call");
+    // (no keys at all: the kernel still writes zeros, and reads none of the one row that it is told of)
+    p.q = q.data_ptr(); p.o = o.data_ptr();
+    p.k = Tk ? k.data_ptr() : q.data_ptr(); p.v = Tk ? v.data_ptr() : q.data_ptr();
+    strides_of(q, p.q_stride);
+    strides_of(o, p.o_stride);
+    if (Tk) {
+        strides_of(k, p.k_stride);
+        strides_of(v, p.v_stride);
+    }
+    p.lse = want_lse ? static_cast<float *>(lse.data_ptr()) : nullptr;
+    p.cu_q = cu_q.const_data_ptr<int32_t>(); p.cu_k = cu_k.const_data_ptr<int32_t>();
+    p.B = (int32_t)B; p.tokens_q = (int32_t)T; p.tokens_k = (int32_t)Tk; p.n_q = (int32_t)n_q; p.n_kv = (int32_t)n_kv; p.head_dim = (int32_t)hd;
+    p.causal = causal ? 1 : 0;
+    check(api.prompt_attention(&p, current_stream(q0)));
+    return with_lse(o, lse);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -791,5 +1030,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("lm_attention", torch::wrap_pybind_function(lm_attention));
     m.def("rotary_pair", torch::wrap_pybind_function(rotary_pair));
     m.def("add_rmsnorm", torch::wrap_pybind_function(add_rmsnorm));
+    m.def("paged_append", torch::wrap_pybind_function(paged_append));
+    m.def("paged_attention", torch::wrap_pybind_function(paged_attention));
+    m.def("prompt_attention", torch::wrap_pybind_function(prompt_attention));
     m.def("rmsnorm", torch::wrap_pybind_function(rmsnorm));
 }

@@ -42,7 +42,8 @@ typedef enum flashmhf_status {
     FLASHMHF_ERR_ARCH = -7,          /* current device is not compute capability 10.x */
     FLASHMHF_ERR_CUDA = -8,          /* a CUDA runtime/driver call failed (see flashmhf_last_cuda_error) */
     FLASHMHF_ERR_DEVICE_TIMEOUT = -9, /* a kernel gave up on a bounded wait and returned early (flashmhf_device_status) */
-    FLASHMHF_ERR_SCRATCH_LIMIT = -10  /* flashmhf_backward_static_scratch: dK, dU, dV in fp32 exceed FLASHMHF_STATIC_SCRATCH_BYTES */
+    FLASHMHF_ERR_SCRATCH_LIMIT = -10, /* flashmhf_backward_static_scratch: dK, dU, dV in fp32 exceed FLASHMHF_STATIC_SCRATCH_BYTES */
+    FLASHMHF_ERR_DEVICE_INDEX = -11   /* a serving kernel met a length or page number out of range and left it out (flashmhf_device_status) */
 } flashmhf_status;
 
 typedef enum flashmhf_dtype {
@@ -268,6 +269,83 @@ int flashmhf_lm_add_rmsnorm_forward(const void *x, const void *d, const void *w,
 int flashmhf_lm_add_rmsnorm_backward(const void *sum, const void *w, int32_t w_dtype, const void *g, const void *g_sum, void *dx, void *dw,
                                      void *workspace, size_t workspace_bytes, int64_t rows, int32_t n, float eps, void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Serving: a key/value cache in pages, held in 8 bits; what writes it, what reads it, and attention over packed prompts.
+ * bf16 activations, head_dim in {64, 96, 128}.  All calls only enqueue work, read lengths and page numbers on the device (so a
+ * captured graph follows them as they change) and allocate nothing.  Reference counterparts: the DynamicCache update and the
+ * attention call of models/flashmhf/modeling_mhffnmoe.py:556-592; the reference has no paged and no 8-bit form.
+ *
+ * One layer's pages.  Code c of page p, key/value head h stands for value(c) * scale[p * n_kv + h], value() the e4m3 number; scales
+ * are powers of two, so that a page whose scale has to grow is rescaled by shifting exponents (exact but for subnormal codes). */
+typedef struct flashmhf_kv_pages {
+    void *k, *v;              /* e4m3 [num_pages][n_kv][page_size][head_dim]; 16-byte aligned; a page is contiguous */
+    float *k_scale, *v_scale; /* [num_pages][n_kv] */
+    int64_t page_stride;      /* bytes from a page to the next, the same for k and v; a multiple of 16 */
+    int32_t num_pages, n_kv, page_size, head_dim; /* page_size in {16, 32, 64, 128} */
+} flashmhf_kv_pages;
+
+/* Which pages the sequences have: position p of sequence b lies in row p % page_size of page table[b * table_stride + p / page_size]. */
+typedef struct flashmhf_kv_sequences {
+    const int32_t *lengths; /* [B] */
+    const int32_t *table;   /* [B][max_pages]; entries behind a sequence's last page are not read */
+    int64_t table_stride;   /* elements, >= max_pages */
+    int32_t B, max_pages;
+} flashmhf_kv_sequences;
+
+/* Rotates the queries and keys of new tokens and puts the keys and values into the pages, one launch.
+ * lengths[b] is what sequence b held BEFORE the call; its new tokens are rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of q, k, v (with
+ * cu_seqlens NULL: row b, one token a sequence) and take positions lengths[b], lengths[b]+1, ...  Rotation: the two halves of a head,
+ * fp32, y1 = x1 c - x2 s, y2 = x2 c + x1 s with row `position` of the tables.  Scale of a page and head: the smallest power of two
+ * (>= 2^-60) with which the largest finite new value is at most 448, at least the page's scale if the page held rows of this sequence
+ * already (those are rescaled when it grows).  NaN and infinities are held as NaN.  A page that is written belongs to one sequence.
+ * q may be NULL (no queries); k_out may be NULL (the rotated keys in bf16, for attention over the prompt itself).  q_out and k_out are
+ * contiguous [tokens][heads][head_dim]; rows of no sequence are left as they are. */
+typedef struct flashmhf_paged_append_params {
+    flashmhf_kv_pages pages;
+    flashmhf_kv_sequences seq;
+    const int32_t *cu_seqlens;        /* [B+1] or NULL */
+    const void *q, *k, *v;            /* bf16 [tokens][n_q | n_kv][head_dim], innermost contiguous, 16-byte aligned */
+    int64_t q_stride[2], k_stride[2], v_stride[2]; /* elements: token, head; multiples of 8 */
+    void *q_out, *k_out;
+    const float *cos_t, *sin_t;       /* [max_positions][head_dim / 2] */
+    int32_t tokens, n_q, max_positions;
+} flashmhf_paged_append_params;
+int flashmhf_paged_append(const flashmhf_paged_append_params *p, void *stream);
+
+/* o[b,i,h] = sum_p softmax_p(scale q[b,i,h].k[p]) v[p] over the first lengths[b] - (n_new-1-i) positions of the pages, for the n_new
+ * newest tokens of each sequence (they are in the pages already); query head h reads key/value head h / (n_q / n_kv).  A row that sees
+ * nothing gives zeros (and -inf).  q, o bf16 [B][n_new][n_q][head_dim]; lse, if not NULL, fp32 [B][n_new][n_q] contiguous: the natural
+ * logarithm of the sum of exponentials.  Workspace: 256-byte aligned, contents undefined before and after; two calls that may run at
+ * the same time need one each.  Deterministic. */
+typedef struct flashmhf_paged_attention_params {
+    flashmhf_kv_pages pages;
+    flashmhf_kv_sequences seq;
+    const void *q;
+    void *o;
+    int64_t q_stride[3], o_stride[3]; /* elements: sequence, new token, head; multiples of 8 */
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t n_q, n_new;               /* n_new in 1 .. 16 */
+    float scale;
+} flashmhf_paged_attention_params;
+size_t flashmhf_paged_attention_workspace_bytes(const flashmhf_paged_attention_params *p);
+int flashmhf_paged_attention(const flashmhf_paged_attention_params *p, void *stream);
+
+/* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1]-1 of q attend to rows cu_k[b] .. cu_k[b+1]-1 of k and v; causal: row r of
+ * the lq rows sees key c of the lk keys where c <= r + lk - lq.  A row that sees nothing gives zeros (and -inf); rows of no sequence
+ * are left as they are.  lse, if not NULL, fp32 [tokens_q][n_q] contiguous. */
+typedef struct flashmhf_prompt_attention_params {
+    const void *q, *k, *v;            /* bf16 [tokens_q | tokens_k][n_q | n_kv][head_dim], innermost contiguous, 16-byte aligned */
+    void *o;                          /* bf16 [tokens_q][n_q][head_dim] */
+    int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2]; /* elements: token, head; multiples of 8 */
+    float *lse;
+    const int32_t *cu_q, *cu_k;       /* [B+1] */
+    int32_t B, tokens_q, tokens_k, n_q, n_kv, head_dim, causal;
+    float scale;
+} flashmhf_prompt_attention_params;
+int flashmhf_prompt_attention(const flashmhf_prompt_attention_params *p, void *stream);
+
 /* SYNCHRONOUS.  Waits for the current device, then reads and clears the status word the kernels
  * write when a bounded wait runs out.  *code = 0 if none did; otherwise a kernel/role identifier
  * (kernel * 100 + wait), and the call returns FLASHMHF_ERR_DEVICE_TIMEOUT.
@@ -277,6 +355,8 @@ int flashmhf_lm_add_rmsnorm_backward(const void *sum, const void *w, int32_t w_d
  * launches are not affected: they run normally whether or not the word has been read.  Because the
  * entry points only enqueue work they cannot report the condition themselves; call this wherever the
  * host already synchronises (after reading back a loss, at the end of a step).
+ * The serving kernels use the same word for what they can see on the device alone: a page number, length or position out of range
+ * is left out (nothing is read or written there), and the call returns FLASHMHF_ERR_DEVICE_INDEX with the kernel's code.
  * Reference counterpart: none. */
 int flashmhf_device_status(int *code);
 
