@@ -1,8 +1,36 @@
 // Attention of the newest tokens of each sequence over its pages of the 8-bit cache.
+//
+// Every code is read once and used by up to eight query rows (the query heads of a key/value head, times the new tokens), so the call
+// is bound by HBM as soon as the cache is larger than a few MB; below that by the chain of dependent loads (lengths, page numbers,
+// scales, codes) and its two launches.
+//
+// Splitting.  The tokens of all (sequence, key/value head, eight query rows) are laid end to end in units of 64 and dealt out to all warps of the
+// GPU in equal contiguous runs, by lengths that only the device knows: one long sequence and a hundred short ones load the machine alike.
+// A warp works alone, from global memory to registers.  A run that covers all of an item writes its rows; else the warp writes its part
+// (at most two a warp: the ends of its run) with its maximum and sum, and a second kernel adds the parts in the order of the tokens.
+//
+// Products.  16 tokens at a time, on mma.m16n8k16 in fp16 with fp32 accumulators: S^T = K Q^T (tokens x rows), O^T += V^T P^T
+// (dims x rows): tokens and dims fill the 16 of a tile, and the few query rows its 8 columns (tcgen05 tiles have at least 64 or 128 of
+// them, and one operand of each product would have to be converted into shared memory).  e4m3 is exact in fp16; queries are scaled by a power of two so that their
+// largest is between 2^14 and 2^15: exact down to 2^-28 of it.  P is rounded to 11 bits; maxima, sums and O are fp32.
+// Which dims a lane's share of a fragment stands for is free as long as both operands agree, so a lane loads HD / 4 neighbouring codes of a
+// key and HD / 8 of a value, straight into fragments; pairs of tokens that V needs side by side are made by byte permutation.
 #include "paged.cuh"
+#include "tc_common.cuh"
 
 namespace fmhf {
 namespace {
+
+constexpr int kUnit = 64;            // tokens
+constexpr int kCols = 8;             // query rows of an item
+constexpr int kWarps = 4;            // of a block; they have nothing to do with one another
+__host__ __device__ constexpr int blocks_per_sm(int hd) { return hd == 64 ? 4 : 3; }      // 128 or 168 registers a thread
+// Weights are kept as P = 2^(s + e - m), 2^e the scale of the values' page: P V is then a product of P and bare codes.  m is set so that the
+// largest P is 2^7, and set again when one exceeds 2^15: fp16 holds P to 11 bits down to 2^-21 of the largest product of weight and
+// scale, and in steps of 2^-31 of it below.  e is kept within +-45 (what a scale is beyond that multiplies the product instead), so that
+// the sum of the weights themselves, P 2^-e, loses nothing in fp32 to pages whose values are larger.
+constexpr float kTop = 7.f, kLazyMax = 15.f;
+constexpr int kMaxExp = 45;
 
 struct PagedArgs {
     const uint8_t *k, *v;
@@ -14,63 +42,402 @@ struct PagedArgs {
     __nv_bfloat16 *o;
     long long q_stride[3], o_stride[3];
     float *lse;
+    float *part;                     // [worker][2][kCols][HD] sums of a warp's parts
+    float2 *ml;                      // [worker][2][kCols] their maxima and sums of weights
+    int4 *shared_by;                 // [item]: first and last worker of it, and which part of the first one's
     int *status;
-    int B, max_pages, num_pages, n_kv, n_q, n_new, P;
-    float scale;
+    int B, max_pages, num_pages, n_kv, n_q, n_new, log_page, group, col_tiles, workers;
+    float c;                         // scale * log2(e)
 };
 
-__device__ __forceinline__ float code_value(uint8_t c) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half_pair(uint32_t two_codes) {      // the codes in the lower 16 bits
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two_codes));
+    return r;
+}
+__device__ __forceinline__ uint32_t half_pair_hi(uint32_t codes) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(codes));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t r) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(r));
+    return d;
+}
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// W words from an address that is a multiple of 4 W bytes where W is a power of two, of 8 for W = 6, of 4 for W = 3.
+template <int W>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[W]) {
+    if constexpr (W % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (W % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+            w[2 * i] = v.x; w[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+    }
 }
 
-// One warp a row (sequence, new token, query head); lane l holds the output's elements l, l + 32, ...
-template <int HD>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const PagedArgs a) {
-    constexpr int N = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (long long)a.B * a.n_new * a.n_q) return;
-    const int h = (int)(row % a.n_q), i = (int)(row / a.n_q % a.n_new), b = (int)(row / a.n_q / a.n_new), kh = h / (a.n_q / a.n_kv);
-    float q[N], o[N] = {};
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-        q[n] = __bfloat162float(a.q[b * a.q_stride[0] + i * a.q_stride[1] + h * a.q_stride[2] + n * 32 + lane]);
-    long long len = a.lengths[b];
-    if (len > (long long)a.max_pages * a.P) {
-        note_index(a.status, kPagedAttnLength);
-        len = (long long)a.max_pages * a.P;
-    }
-    len -= a.n_new - 1 - i;
-    float m = -INFINITY, l = 0.f;
-    for (long long p = 0; p < len; ++p) {
-        const int page = a.table[b * a.table_stride + p / a.P];
-        if (page < 0 || page >= a.num_pages) {
-            note_index(a.status, kPagedAttnPage);
-            continue;
-        }
-        const long long at = page * a.page_stride + ((long long)kh * a.P + p % a.P) * HD + lane;
-        float s = 0.f;
-#pragma unroll
-        for (int n = 0; n < N; ++n) s += q[n] * code_value(a.k[at + n * 32]);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= a.k_scale[(long long)page * a.n_kv + kh] * a.scale;
-        const float now = fmaxf(m, s), keep = expf(m - now), w = expf(s - now), wv = w * a.v_scale[(long long)page * a.n_kv + kh];
-        m = now;
-        l = l * keep + w;
-#pragma unroll
-        for (int n = 0; n < N; ++n) o[n] = o[n] * keep + wv * code_value(a.v[at + n * 32]);
-    }
-    const float r = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-        a.o[b * a.o_stride[0] + i * a.o_stride[1] + h * a.o_stride[2] + n * 32 + lane] = __float2bfloat16(o[n] * r);
-    if (a.lse && lane == 0) a.lse[row] = l > 0.f ? m + logf(l) : -INFINITY;
+// Tokens in the cache of sequence b, as far as its row of the table goes.
+__device__ __forceinline__ int length_of(const PagedArgs &a, int b) {
+    const int n = __ldg(a.lengths + b);
+    const long long most = (long long)a.max_pages << a.log_page;
+    if (n > most) note_index(a.status, kPagedAttnLength);
+    return max(0, (int)min((long long)n, most));
 }
+__device__ __forceinline__ long long units_of(int len) { return (len + kUnit - 1) / kUnit; }
+__device__ __forceinline__ long long warp_sum(long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Units of an item of each sequence, summed over sequences first .. last - 1 (a whole warp asks).
+__device__ long long units_between(const PagedArgs &a, int first, int last) {
+    long long n = 0;
+    for (int b = first + (threadIdx.x & 31); b < last; b += 32) n += units_of(length_of(a, b));
+    return warp_sum(n);
+}
+
+template <int HD>
+struct Step {                        // the codes of 16 tokens, a lane's share
+    uint32_t k[2][HD / 16], v[4][HD / 32];
+    float ks, ve, vr;                // key scale, exponent of the value scale (clamped), the rest of it
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attention_kernel(const PagedArgs a) {
+    constexpr int KK = HD / 16, MT = HD / 16;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int worker = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int per_seq = a.n_kv * a.col_tiles, P = 1 << a.log_page, rows = a.group * a.n_new;
+    const long long total = units_between(a, 0, a.B) * per_seq;
+    griddep_launch_dependents();
+    const int workers = (int)min((long long)a.workers, total);       // each has a unit at least
+    if (worker >= workers) return;
+    long long u = total * worker / workers;
+    const long long u_end = total * (worker + 1) / workers, u_first = u;
+
+    // the sequence that unit u belongs to, and where its units begin
+    int b = 0;
+    long long base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        long long n = b0 + lane < a.B ? units_of(length_of(a, b0 + lane)) * per_seq : 0, sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, base + sum > u);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            b = b0 + at;
+            base += __shfl_sync(0xffffffffu, sum - n, at);
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+
+    while (u < u_end) {
+        int len = length_of(a, b);
+        long long n_units = units_of(len);
+        while (u >= base + n_units * per_seq) {         // (sequences without tokens are passed over)
+            base += n_units * per_seq;
+            len = length_of(a, ++b);
+            n_units = units_of(len);
+        }
+        const int item = (int)((u - base) / n_units), head = item / a.col_tiles, col0 = (item % a.col_tiles) * kCols;
+        const long long begin = base + item * n_units, end = begin + n_units, stop = min(end, u_end);
+        const int tok0 = (int)(u - begin) * kUnit, tok1 = (int)min((long long)len, (stop - begin) * kUnit);
+
+        // queries: column g of the tile, dims HD / 4 * t on
+        uint32_t qf[KK][2];
+        float fac[2];                                    // what scores of columns 2t, 2t + 1 are multiplied by
+        {
+            const int r = col0 + g;
+            float x[HD / 4], top = 0.f;
+            if (r < rows) {
+                const __nv_bfloat16 *q = a.q + b * a.q_stride[0] + (r / a.group) * a.q_stride[1] + (head * a.group + r % a.group) * a.q_stride[2] + t * (HD / 4);
+                uint32_t w[HD / 8];
+                load_words<HD / 8>(reinterpret_cast<const uint8_t *>(q), w);
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) {
+                    x[2 * i] = __uint_as_float(w[i] << 16);
+                    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < HD / 4; ++i) x[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^14 over the power of two in `top`, and its inverse; both normal numbers (top below 2^-112 loses bits that no score shows)
+            const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 254);
+            const float up = __uint_as_float((uint32_t)(254 + 14 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
+#pragma unroll
+            for (int i = 0; i < KK; ++i) {
+                qf[i][0] = pack_half(x[4 * i] * up, x[4 * i + 1] * up);
+                qf[i][1] = pack_half(x[4 * i + 2] * up, x[4 * i + 3] * up);
+            }
+            fac[0] = a.c * __shfl_sync(0xffffffffu, down, 8 * t);
+            fac[1] = a.c * __shfl_sync(0xffffffffu, down, 8 * t + 4);
+        }
+        // tokens that the lane's columns see
+        int see[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) see[i] = len - (a.n_new - 1 - min(rows - 1, col0 + 2 * t + i) / a.group);
+        const int all = len - (a.n_new - 1);
+
+        // pages: lane i knows page first_page + i and its scales, and those of the 32 after
+        const int32_t *table = a.table + b * a.table_stride;
+        const int last_page = (tok1 - 1) >> a.log_page;
+        int page_base = tok0 >> a.log_page;
+        int id, id2;
+        float ks, ve, vr, ks2, ve2, vr2;
+        auto pages = [&](int first, int &pid, float &k, float &e, float &r) {
+            pid = first + lane <= last_page ? __ldg(table + first + lane) : -1;
+            if (first + lane <= last_page && (pid < 0 || pid >= a.num_pages)) {
+                note_index(a.status, kPagedAttnPage);
+                pid = -1;
+            }
+            k = e = 0.f;
+            r = 1.f;
+            if (pid >= 0) {
+                k = __ldg(a.k_scale + (long long)pid * a.n_kv + head);
+                const float v = __ldg(a.v_scale + (long long)pid * a.n_kv + head);
+                const int n = min(max((int)(__float_as_uint(v) >> 23 & 255) - 127, -kMaxExp), kMaxExp);
+                e = (float)n;
+                r = v * __uint_as_float((uint32_t)(127 - n) << 23);
+            }
+        };
+        pages(page_base, id, ks, ve, vr);
+        pages(page_base + 32, id2, ks2, ve2, vr2);
+
+        float o[MT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        auto load = [&](int tok, Step<HD> &s) {          // the 16 tokens from `tok` on (all of one page)
+            int pi = (tok >> a.log_page) - page_base;
+            if (pi >= 32) {
+                id = id2; ks = ks2; ve = ve2; vr = vr2;
+                page_base += 32;
+                pi -= 32;
+                pages(page_base + 32, id2, ks2, ve2, vr2);
+            }
+            const int pid = __shfl_sync(0xffffffffu, id, pi);
+            s.ks = __shfl_sync(0xffffffffu, ks, pi);
+            s.ve = __shfl_sync(0xffffffffu, ve, pi);
+            s.vr = __shfl_sync(0xffffffffu, vr, pi);
+            const int left = pid < 0 ? 0 : tok1 - tok;    // tokens of the 16 that are there
+            if (pid < 0) s.ks = NAN;                      // (none of them: see `compute`)
+            const long long at = (long long)max(pid, 0) * a.page_stride + ((long long)head * P + (tok & (P - 1))) * HD;
+            const uint8_t *k = a.k + at + t * (HD / 4), *v = a.v + at + g * (HD / 8);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (g + 8 * i < left) load_words<HD / 16>(k + (g + 8 * i) * HD, s.k[i]);
+                else
+#pragma unroll
+                    for (int w = 0; w < HD / 16; ++w) s.k[i][w] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int x = 2 * t + (i & 1) + 8 * (i >> 1);
+                if (x < left) load_words<HD / 32>(v + x * HD, s.v[i]);
+                else
+#pragma unroll
+                    for (int w = 0; w < HD / 32; ++w) s.v[i][w] = 0;
+            }
+        };
+        auto compute = [&](int tok, const Step<HD> &st) {
+            float s[4] = {};
+#pragma unroll
+            for (int i = 0; i < KK; ++i)
+                mma16(s, half_pair(st.k[0][i]), half_pair(st.k[1][i]), half_pair_hi(st.k[0][i]), half_pair_hi(st.k[1][i]), qf[i][0], qf[i][1]);
+            const bool none = st.ks != st.ks;
+            const float f0 = fac[0] * st.ks, f1 = fac[1] * st.ks;
+            s[0] = fmaf(s[0], f0, st.ve); s[1] = fmaf(s[1], f1, st.ve); s[2] = fmaf(s[2], f0, st.ve); s[3] = fmaf(s[3], f1, st.ve);
+            if (tok + 16 > min(all, tok1) || none) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (none || tok + g + 8 * (i >> 1) >= min(see[i & 1], tok1)) s[i] = -INFINITY;
+            }
+            const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+            if (__any_sync(0xffffffffu, x0 - m[0] > kLazyMax || x1 - m[1] > kLazyMax)) {
+                float n0 = x0, n1 = x1;
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
+                    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
+                }
+                // (a column whose maximum has not grown, or that has seen nothing, keeps what it has)
+                n0 = n0 - kTop > m[0] ? n0 - kTop : m[0];
+                n1 = n1 - kTop > m[1] ? n1 - kTop : m[1];
+                const float k0 = m[0] == n0 ? 1.f : ex2(m[0] - n0), k1 = m[1] == n1 ? 1.f : ex2(m[1] - n1);
+                m[0] = n0; m[1] = n1;
+                l[0] *= k0; l[1] *= k1;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) { o[i][0] *= k0; o[i][1] *= k1; o[i][2] *= k0; o[i][3] *= k1; }
+            }
+            const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+            s[0] = ex2(s[0] - m0); s[1] = ex2(s[1] - m1); s[2] = ex2(s[2] - m0); s[3] = ex2(s[3] - m1);
+            const float weigh = __uint_as_float((uint32_t)(127 - (int)st.ve) << 23);
+            l[0] = fmaf(s[0] + s[2], weigh, l[0]);
+            l[1] = fmaf(s[1] + s[3], weigh, l[1]);
+            const uint32_t p0 = transpose8x8(pack_half(s[0], s[1])), p1 = transpose8x8(pack_half(s[2], s[3]));
+            const bool plain = st.vr == 1.f;
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x = __byte_perm(st.v[0][w], st.v[1][w], h ? 0x7362 : 0x5140), y = __byte_perm(st.v[2][w], st.v[3][w], h ? 0x7362 : 0x5140);
+                    if (plain) {
+                        mma16(o[2 * w + h], half_pair(x), half_pair_hi(x), half_pair(y), half_pair_hi(y), p0, p1);
+                    } else {
+                        float d[4] = {};
+                        mma16(d, half_pair(x), half_pair_hi(x), half_pair(y), half_pair_hi(y), p0, p1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[2 * w + h][i] = fmaf(d[i], st.vr, o[2 * w + h][i]);
+                    }
+                }
+            }
+        };
+        Step<HD> s0, s1;
+        load(tok0, s0);
+        for (int tok = tok0; tok < tok1; tok += 32) {
+            if (tok + 16 < tok1) load(tok + 16, s1);
+            compute(tok, s0);
+            if (tok + 16 >= tok1) break;
+            if (tok + 32 < tok1) load(tok + 32, s0);
+            compute(tok + 16, s1);
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
+        }
+        if (u == begin && stop == end) {                 // all of the item
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = col0 + 2 * t + i;
+                if (r >= rows) continue;
+                const int n = r / a.group, h = head * a.group + r % a.group;
+                const float f = l[i] == 0.f ? 0.f : 1.f / l[i];
+                uint32_t *dst = reinterpret_cast<uint32_t *>(a.o + b * a.o_stride[0] + n * a.o_stride[1] + h * a.o_stride[2] + g * (HD / 8));
+#pragma unroll
+                for (int x = 0; x < MT; ++x) {
+                    const __nv_bfloat162 y = __floats2bfloat162_rn(l[i] == 0.f ? 0.f : o[x][i] * f, l[i] == 0.f ? 0.f : o[x][i + 2] * f);
+                    dst[x] = *reinterpret_cast<const uint32_t *>(&y);
+                }
+                if (a.lse && g == 0) a.lse[((long long)b * a.n_new + n) * a.n_q + h] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * 0.6931471805599453f;
+            }
+        } else {
+            const int slot = u == u_first ? 0 : 1;
+            const long long at = ((long long)worker * 2 + slot) * kCols;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int cidx = 2 * t + i;
+                if (col0 + cidx >= rows) continue;
+                float2 *dst = reinterpret_cast<float2 *>(a.part + (at + cidx) * HD + g * (HD / 8));
+#pragma unroll
+                for (int x = 0; x < MT; ++x) dst[x] = make_float2(o[x][i], o[x][i + 2]);
+                if (g == 0) a.ml[at + cidx] = make_float2(m[i], l[i]);
+            }
+        }
+        if (stop == end && lane == 0) {
+            // the worker of unit x is the last w with floor(w total / workers) <= x
+            const int w0 = (int)(((begin + 1) * workers - 1) / total);
+            a.shared_by[(long long)b * per_seq + item] = make_int4(w0, worker, total * w0 / workers < begin ? 1 : 0, 0);
+        }
+        u = stop;
+    }
+}
+
+// The parts of items that more than one worker had, added in the order of the tokens (each of a block's warps every fourth of them, then the four sums);
+// and rows of sequences without tokens.  A block a row; a lane holds dims l, l + 32, ...
+constexpr int kCombineWarps = 4;
+template <int HD>
+__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const PagedArgs a) {
+    constexpr int N = HD / 32;
+    __shared__ float sum[kCombineWarps][HD], top[kCombineWarps], weights[kCombineWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = a.group * a.n_new;
+    const int r = (int)(blockIdx.x % rows), head = (int)(blockIdx.x / rows % a.n_kv), b = (int)(blockIdx.x / rows / a.n_kv);
+    const int n = r / a.group, h = head * a.group + r % a.group, col = r % kCols;
+    const bool empty = length_of(a, b) == 0;
+    griddep_wait();        // launched early, behind the kernel whose parts it adds
+    const int4 by = empty ? make_int4(0, 0, 0, 0) : a.shared_by[((long long)b * a.n_kv + head) * a.col_tiles + r / kCols];
+    if (!empty && by.x == by.y) return;
+    auto at = [&](int w) { return ((long long)w * 2 + (w == by.x ? by.z : 0)) * kCols + col; };
+    float m = -INFINITY, l = 0.f, o[N] = {};
+    if (!empty) {
+        for (int w = by.x + threadIdx.x; w <= by.y; w += kCombineWarps * 32) m = fmaxf(m, a.ml[at(w)].x);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        if (lane == 0) top[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kCombineWarps; ++i) m = fmaxf(m, top[i]);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+        for (int w = by.x + warp; w <= by.y; w += kCombineWarps) {
+            const long long i = at(w);
+            const float2 ml = a.ml[i];
+            const float f = ex2(ml.x - ref);
+            l = fmaf(ml.y, f, l);
+#pragma unroll
+            for (int x = 0; x < N; ++x) o[x] = fmaf(a.part[i * HD + x * 32 + lane], f, o[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < N; ++x) sum[warp][x * 32 + lane] = o[x];
+        if (lane == 0) weights[warp] = l;
+        __syncthreads();
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < kCombineWarps; ++i) l += weights[i];
+    }
+    __nv_bfloat16 *dst = a.o + b * a.o_stride[0] + n * a.o_stride[1] + h * a.o_stride[2];
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    for (int d = threadIdx.x; d < HD; d += kCombineWarps * 32) {
+        float y = 0.f;
+        if (!empty)
+#pragma unroll
+            for (int i = 0; i < kCombineWarps; ++i) y += sum[i][d];
+        dst[d] = __float2bfloat16(l == 0.f ? 0.f : y * f);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[((long long)b * a.n_new + n) * a.n_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+int workers_for(int num_sms, int hd) { return num_sms * blocks_per_sm(hd) * kWarps; }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(const flashmhf_paged_attention_params &) { return 0; }
+int col_tiles_of(const flashmhf_paged_attention_params &p) { return (p.n_q / p.pages.n_kv * p.n_new + kCols - 1) / kCols; }
+
+size_t paged_attention_workspace_bytes(const flashmhf_paged_attention_params &p) {
+    return (size_t)workers_for(num_sms(), p.pages.head_dim) * 2 * kCols * (p.pages.head_dim + 2) * sizeof(float) +
+           (size_t)p.seq.B * p.pages.n_kv * col_tiles_of(p) * sizeof(int4);
+}
 
 int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &ctl, cudaStream_t st, int *n_launch) {
     PagedArgs a{};
@@ -81,17 +448,26 @@ int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &c
     a.q = static_cast<const __nv_bfloat16 *>(p.q); a.o = static_cast<__nv_bfloat16 *>(p.o);
     for (int i = 0; i < 3; ++i) { a.q_stride[i] = p.q_stride[i]; a.o_stride[i] = p.o_stride[i]; }
     a.lse = p.lse; a.status = ctl.status;
-    a.B = p.seq.B; a.max_pages = p.seq.max_pages; a.num_pages = g.num_pages; a.n_kv = g.n_kv; a.n_q = p.n_q; a.n_new = p.n_new; a.P = g.page_size;
-    a.scale = p.scale;
+    a.B = p.seq.B; a.max_pages = p.seq.max_pages; a.num_pages = g.num_pages; a.n_kv = g.n_kv; a.n_q = p.n_q; a.n_new = p.n_new;
+    a.log_page = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
+    a.group = p.n_q / g.n_kv;
+    a.col_tiles = col_tiles_of(p);
+    a.workers = workers_for(ctl.num_sms, g.head_dim);
+    a.part = static_cast<float *>(p.workspace);
+    a.ml = reinterpret_cast<float2 *>(a.part + (size_t)a.workers * 2 * kCols * g.head_dim);
+    a.shared_by = reinterpret_cast<int4 *>(a.ml + (size_t)a.workers * 2 * kCols);
+    a.c = p.scale * 1.4426950408889634f;
     const long long rows = (long long)a.B * a.n_new * a.n_q;
-    if ((rows + 3) / 4 > 0x7fffffffll) return FLASHMHF_ERR_BAD_SHAPE;
+    if (rows > 0x7fffffffll) return FLASHMHF_ERR_BAD_SHAPE;
     auto kernel = g.head_dim == 64 ? paged_attention_kernel<64> : g.head_dim == 96 ? paged_attention_kernel<96> : paged_attention_kernel<128>;
-    const cudaError_t e = launch_kernel(false, kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a);
+    auto combine = g.head_dim == 64 ? paged_combine_kernel<64> : g.head_dim == 96 ? paged_combine_kernel<96> : paged_combine_kernel<128>;
+    cudaError_t e = launch_kernel(false, kernel, dim3((unsigned)(a.workers / kWarps)), dim3(kWarps * 32), 0, st, a);
+    if (e == cudaSuccess) e = launch_kernel(true, combine, dim3((unsigned)rows), dim3(kCombineWarps * 32), 0, st, a);
     if (e != cudaSuccess) {
         set_cuda_error(e, "paged attention launch");
         return FLASHMHF_ERR_CUDA;
     }
-    ++*n_launch;
+    *n_launch += 2;
     return FLASHMHF_OK;
 }
 
