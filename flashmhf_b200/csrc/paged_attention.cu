@@ -6,8 +6,10 @@
 //
 // Splitting.  The tokens of all (sequence, key/value head, eight query rows) are laid end to end in units of 64 and dealt out to all warps of the
 // GPU in equal contiguous runs, by lengths that only the device knows: one long sequence and a hundred short ones load the machine alike.
-// A warp works alone, from global memory to registers.  A run that covers all of an item writes its rows; else the warp writes its part
-// (at most two a warp: the ends of its run) with its maximum and sum, and a second kernel adds the parts in the order of the tokens.
+// A warp works alone: its codes come by bulk copies into a ring of its own in shared memory (12 KB a warp, 192 KB in flight on an SM: what
+// 6.5 TB/s at over a microsecond's latency take; with the next 16 tokens in registers it was a third less), and go from there into fragments.
+// A run that covers all of an item writes its rows; else the warp writes its part (at most two a warp: the ends of its run) with its maximum
+// and sum, and a second kernel adds the parts in the order of the tokens.
 //
 // Products.  16 tokens at a time, on mma.m16n8k16 in fp16 with fp32 accumulators: S^T = K Q^T (tokens x rows), O^T += V^T P^T
 // (dims x rows): tokens and dims fill the 16 of a tile, and the few query rows its 8 columns (tcgen05 tiles have at least 64 or 128 of
@@ -24,7 +26,14 @@ namespace {
 constexpr int kUnit = 64;            // tokens
 constexpr int kCols = 8;             // query rows of an item
 constexpr int kWarps = 4;            // of a block; they have nothing to do with one another
-__host__ __device__ constexpr int blocks_per_sm(int hd) { return hd == 64 ? 4 : 3; }      // 128 or 168 registers a thread
+constexpr int kBlocksPerSm = 4;
+constexpr int kKernelPaged = 7;      // status codes 701..
+template <int HD>
+struct Ring {
+    static constexpr int kTokens = HD == 64 ? 32 : 16, kStages = HD == 96 ? 4 : 3;       // of a stage; 12 KB in all
+    static constexpr uint32_t kHalf = kTokens * HD, kStage = 2 * kHalf;                 // keys, then values
+    static constexpr uint32_t kBytes = kStages * kStage;
+};
 // Weights are kept as P = 2^(s + e - m), 2^e the scale of the values' page: P V is then a product of P and bare codes.  m is set so that the
 // largest P is 2^7, and set again when one exceeds 2^15: fp16 holds P to 11 bits down to 2^-21 of the largest product of weight and
 // scale, and in steps of 2^-31 of it below.  e is kept within +-45 (what a scale is beyond that multiplies the product instead), so that
@@ -48,6 +57,7 @@ struct PagedArgs {
     int *status;
     int B, max_pages, num_pages, n_kv, n_q, n_new, log_page, group, col_tiles, workers;
     float c;                         // scale * log2(e)
+    WaitArgs wait;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -80,24 +90,28 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 // W words from an address that is a multiple of 4 W bytes where W is a power of two, of 8 for W = 6, of 4 for W = 3.
 template <int W>
 __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[W]) {
     if constexpr (W % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < W / 4; ++i) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            const uint4 v = *(reinterpret_cast<const uint4 *>(p) + i);
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
     } else if constexpr (W % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < W / 2; ++i) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+            const uint2 v = *(reinterpret_cast<const uint2 *>(p) + i);
             w[2 * i] = v.x; w[2 * i + 1] = v.y;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+        for (int i = 0; i < W; ++i) w[i] = *(reinterpret_cast<const uint32_t *>(p) + i);
     }
 }
 
@@ -121,20 +135,34 @@ __device__ long long units_between(const PagedArgs &a, int first, int last) {
     return warp_sum(n);
 }
 
-template <int HD>
-struct Step {                        // the codes of 16 tokens, a lane's share
-    uint32_t k[2][HD / 16], v[4][HD / 32];
-    float ks, ve, vr;                // key scale, exponent of the value scale (clamped), the rest of it
+// What a stage's pages stand for, by its 16 tokens: key scale (NaN: no page), exponent of the value scale (clamped), the rest of that scale.
+struct Granule {
+    float ks, ve, vr, pad;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attention_kernel(const PagedArgs a) {
-    constexpr int KK = HD / 16, MT = HD / 16;
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_kernel(const PagedArgs a) {
+    using R = Ring<HD>;
+    constexpr int KK = HD / 16, MT = HD / 16, NS = R::kStages, NG = R::kTokens / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) unsigned long long bars[kWarps][NS];
+    __shared__ Granule granules[kWarps][NS][NG];
+    __shared__ int abort_flag;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int worker = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int warp = threadIdx.x >> 5;
+    const uint8_t *ring = smem + warp * R::kBytes;
+    const uint32_t ring_at = smem_u32(ring), bar_at = smem_u32(&bars[warp][0]);
+    const WaitCtl ctl{&abort_flag, a.wait};
+    if (threadIdx.x == 0) abort_flag = launch_aborted(a.wait);
+    if (lane < NS) mbar_init(bar_at + 8 * lane, 1);
+    fence_mbar_init();
+    __syncthreads();
+    griddep_launch_dependents();
+    if (abort_flag) return;
+    uint32_t issued = 0, used = 0;      // stages, counted through all of the run
     const int per_seq = a.n_kv * a.col_tiles, P = 1 << a.log_page, rows = a.group * a.n_new;
     const long long total = units_between(a, 0, a.B) * per_seq;
-    griddep_launch_dependents();
     const int workers = (int)min((long long)a.workers, total);       // each has a unit at least
     if (worker >= workers) return;
     long long u = total * worker / workers;
@@ -238,50 +266,71 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attentio
         pages(page_base + 32, id2, ks2, ve2, vr2);
 
         float o[MT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        auto load = [&](int tok, Step<HD> &s) {          // the 16 tokens from `tok` on (all of one page)
-            int pi = (tok >> a.log_page) - page_base;
-            if (pi >= 32) {
-                id = id2; ks = ks2; ve = ve2; vr = vr2;
-                page_base += 32;
-                pi -= 32;
-                pages(page_base + 32, id2, ks2, ve2, vr2);
+        // Copies of the stage of tokens from `tok` on.  The warp has read what was there (it meets before each call).
+        auto load = [&](int tok) {
+            const uint32_t st = issued++ % NS, dst = ring_at + st * R::kStage, bar = bar_at + 8 * st;
+            const int n = min(R::kTokens, (tok1 - tok + 15) & ~15), step = min(P, n);       // whole 16s: rows of a page exist, used or not
+            int pid[NG];
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                pid[i] = -1;
+                if (i * 16 < n) {
+                    int pi = ((tok + i * 16) >> a.log_page) - page_base;
+                    if (pi >= 32) {
+                        id = id2; ks = ks2; ve = ve2; vr = vr2;
+                        page_base += 32;
+                        pi -= 32;
+                        pages(page_base + 32, id2, ks2, ve2, vr2);
+                    }
+                    pid[i] = __shfl_sync(0xffffffffu, id, pi);
+                    Granule x;
+                    x.ks = __shfl_sync(0xffffffffu, ks, pi);
+                    x.ve = __shfl_sync(0xffffffffu, ve, pi);
+                    x.vr = __shfl_sync(0xffffffffu, vr, pi);
+                    if (pid[i] < 0) x.ks = NAN;
+                    else bytes += 2 * 16 * HD;
+                    if (lane == 0) granules[warp][st][i] = x;
+                }
             }
-            const int pid = __shfl_sync(0xffffffffu, id, pi);
-            s.ks = __shfl_sync(0xffffffffu, ks, pi);
-            s.ve = __shfl_sync(0xffffffffu, ve, pi);
-            s.vr = __shfl_sync(0xffffffffu, vr, pi);
-            const int left = pid < 0 ? 0 : tok1 - tok;    // tokens of the 16 that are there
-            if (pid < 0) s.ks = NAN;                      // (none of them: see `compute`)
-            const long long at = (long long)max(pid, 0) * a.page_stride + ((long long)head * P + (tok & (P - 1))) * HD;
-            const uint8_t *k = a.k + at + t * (HD / 4), *v = a.v + at + g * (HD / 8);
+            if (lane == 0) {
+                if (bytes) mbar_arrive_expect_tx(bar, bytes);
+                else mbar_arrive(bar);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (g + 8 * i < left) load_words<HD / 16>(k + (g + 8 * i) * HD, s.k[i]);
-                else
-#pragma unroll
-                    for (int w = 0; w < HD / 16; ++w) s.k[i][w] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int x = 2 * t + (i & 1) + 8 * (i >> 1);
-                if (x < left) load_words<HD / 32>(v + x * HD, s.v[i]);
-                else
-#pragma unroll
-                    for (int w = 0; w < HD / 32; ++w) s.v[i][w] = 0;
+                for (int i = 0; i < NG; ++i) {
+                    // (a page of 32 or more holds the stage: one copy of each kind)
+                    if (i * 16 >= n || pid[i] < 0 || (i > 0 && step > 16)) continue;
+                    const long long at = (long long)pid[i] * a.page_stride + ((long long)head * P + ((tok + i * 16) & (P - 1))) * HD;
+                    const uint32_t size = (step > 16 ? n : 16) * HD;
+                    bulk_load(dst + i * 16 * HD, a.k + at, size, bar);
+                    bulk_load(dst + R::kHalf + i * 16 * HD, a.v + at, size, bar);
+                }
             }
         };
-        auto compute = [&](int tok, const Step<HD> &st) {
-            float s[4] = {};
-#pragma unroll
-            for (int i = 0; i < KK; ++i)
-                mma16(s, half_pair(st.k[0][i]), half_pair(st.k[1][i]), half_pair_hi(st.k[0][i]), half_pair_hi(st.k[1][i]), qf[i][0], qf[i][1]);
+        auto compute = [&](int tok, const uint8_t *keys, const Granule st) {
             const bool none = st.ks != st.ks;
+            const int left = none ? 0 : tok1 - tok;       // tokens of the 16 that are there; what lies behind them may be anything
+            float s[4] = {};
+            {
+                uint32_t k0[HD / 16], k1[HD / 16];
+                load_words<HD / 16>(keys + g * HD + t * (HD / 4), k0);
+                load_words<HD / 16>(keys + (g + 8) * HD + t * (HD / 4), k1);
+#pragma unroll
+                for (int i = 0; i < KK; ++i) mma16(s, half_pair(k0[i]), half_pair(k1[i]), half_pair_hi(k0[i]), half_pair_hi(k1[i]), qf[i][0], qf[i][1]);
+            }
+            uint32_t v[4][HD / 32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_words<HD / 32>(keys + R::kHalf + (2 * t + (i & 1) + 8 * (i >> 1)) * HD + g * (HD / 8), v[i]);
             const float f0 = fac[0] * st.ks, f1 = fac[1] * st.ks;
             s[0] = fmaf(s[0], f0, st.ve); s[1] = fmaf(s[1], f1, st.ve); s[2] = fmaf(s[2], f0, st.ve); s[3] = fmaf(s[3], f1, st.ve);
             if (tok + 16 > min(all, tok1) || none) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i) {
                     if (none || tok + g + 8 * (i >> 1) >= min(see[i & 1], tok1)) s[i] = -INFINITY;
+                    if (2 * t + (i & 1) + 8 * (i >> 1) >= left)
+#pragma unroll
+                        for (int w = 0; w < HD / 32; ++w) v[i][w] = 0;
+                }
             }
             const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
             if (__any_sync(0xffffffffu, x0 - m[0] > kLazyMax || x1 - m[1] > kLazyMax)) {
@@ -294,11 +343,11 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attentio
                 // (a column whose maximum has not grown, or that has seen nothing, keeps what it has)
                 n0 = n0 - kTop > m[0] ? n0 - kTop : m[0];
                 n1 = n1 - kTop > m[1] ? n1 - kTop : m[1];
-                const float k0 = m[0] == n0 ? 1.f : ex2(m[0] - n0), k1 = m[1] == n1 ? 1.f : ex2(m[1] - n1);
+                const float f0 = m[0] == n0 ? 1.f : ex2(m[0] - n0), f1 = m[1] == n1 ? 1.f : ex2(m[1] - n1);
                 m[0] = n0; m[1] = n1;
-                l[0] *= k0; l[1] *= k1;
+                l[0] *= f0; l[1] *= f1;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) { o[i][0] *= k0; o[i][1] *= k1; o[i][2] *= k0; o[i][3] *= k1; }
+                for (int i = 0; i < MT; ++i) { o[i][0] *= f0; o[i][1] *= f1; o[i][2] *= f0; o[i][3] *= f1; }
             }
             const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
             s[0] = ex2(s[0] - m0); s[1] = ex2(s[1] - m1); s[2] = ex2(s[2] - m0); s[3] = ex2(s[3] - m1);
@@ -311,7 +360,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attentio
             for (int w = 0; w < HD / 32; ++w) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t x = __byte_perm(st.v[0][w], st.v[1][w], h ? 0x7362 : 0x5140), y = __byte_perm(st.v[2][w], st.v[3][w], h ? 0x7362 : 0x5140);
+                    const uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140), y = __byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140);
                     if (plain) {
                         mma16(o[2 * w + h], half_pair(x), half_pair_hi(x), half_pair(y), half_pair_hi(y), p0, p1);
                     } else {
@@ -323,14 +372,20 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attentio
                 }
             }
         };
-        Step<HD> s0, s1;
-        load(tok0, s0);
-        for (int tok = tok0; tok < tok1; tok += 32) {
-            if (tok + 16 < tok1) load(tok + 16, s1);
-            compute(tok, s0);
-            if (tok + 16 >= tok1) break;
-            if (tok + 32 < tok1) load(tok + 32, s0);
-            compute(tok + 16, s1);
+        for (int i = 0; i < NS; ++i)
+            if (tok0 + i * R::kTokens < tok1) load(tok0 + i * R::kTokens);
+        for (int tok = tok0; tok < tok1; tok += R::kTokens, ++used) {
+            const uint32_t st = used % NS;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar_at + 8 * st, (used / NS) & 1, ctl, kKernelPaged * 100 + 1))) {
+                const long long t_end = clock64() + (1LL << 19);      // copies in flight land before shared memory is given back
+                while (clock64() < t_end) __nanosleep(256);
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < NG; ++i)
+                if (tok + 16 * i < tok1) compute(tok + 16 * i, ring + st * R::kStage + i * 16 * HD, granules[warp][st][i]);
+            __syncwarp();
+            if (tok + NS * R::kTokens < tok1) load(tok + NS * R::kTokens);
         }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
@@ -374,10 +429,10 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD)) paged_attentio
     }
 }
 
-// The parts of items that more than one worker had, added in the order of the tokens (each of a block's warps every fourth of them, then the four sums);
+// The parts of items that more than one worker had, added in the order of the tokens (each of a block's warps every
+// fourth or sixteenth of them, then the warps' sums);
 // and rows of sequences without tokens.  A block a row; a lane holds dims l, l + 32, ...
-constexpr int kCombineWarps = 4;
-template <int HD>
+template <int HD, int kCombineWarps>
 __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const PagedArgs a) {
     constexpr int N = HD / 32;
     __shared__ float sum[kCombineWarps][HD], top[kCombineWarps], weights[kCombineWarps];
@@ -428,14 +483,14 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
     if (a.lse && threadIdx.x == 0) a.lse[((long long)b * a.n_new + n) * a.n_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-int workers_for(int num_sms, int hd) { return num_sms * blocks_per_sm(hd) * kWarps; }
+int workers_for(int num_sms) { return num_sms * kBlocksPerSm * kWarps; }
 
 }  // namespace
 
 int col_tiles_of(const flashmhf_paged_attention_params &p) { return (p.n_q / p.pages.n_kv * p.n_new + kCols - 1) / kCols; }
 
 size_t paged_attention_workspace_bytes(const flashmhf_paged_attention_params &p) {
-    return (size_t)workers_for(num_sms(), p.pages.head_dim) * 2 * kCols * (p.pages.head_dim + 2) * sizeof(float) +
+    return (size_t)workers_for(num_sms()) * 2 * kCols * (p.pages.head_dim + 2) * sizeof(float) +
            (size_t)p.seq.B * p.pages.n_kv * col_tiles_of(p) * sizeof(int4);
 }
 
@@ -452,17 +507,26 @@ int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &c
     a.log_page = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
     a.group = p.n_q / g.n_kv;
     a.col_tiles = col_tiles_of(p);
-    a.workers = workers_for(ctl.num_sms, g.head_dim);
+    a.workers = workers_for(ctl.num_sms);
     a.part = static_cast<float *>(p.workspace);
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)a.workers * 2 * kCols * g.head_dim);
     a.shared_by = reinterpret_cast<int4 *>(a.ml + (size_t)a.workers * 2 * kCols);
     a.c = p.scale * 1.4426950408889634f;
     const long long rows = (long long)a.B * a.n_new * a.n_q;
     if (rows > 0x7fffffffll) return FLASHMHF_ERR_BAD_SHAPE;
+    a.wait = wait_args(&ctl);
     auto kernel = g.head_dim == 64 ? paged_attention_kernel<64> : g.head_dim == 96 ? paged_attention_kernel<96> : paged_attention_kernel<128>;
-    auto combine = g.head_dim == 64 ? paged_combine_kernel<64> : g.head_dim == 96 ? paged_combine_kernel<96> : paged_combine_kernel<128>;
-    cudaError_t e = launch_kernel(false, kernel, dim3((unsigned)(a.workers / kWarps)), dim3(kWarps * 32), 0, st, a);
-    if (e == cudaSuccess) e = launch_kernel(true, combine, dim3((unsigned)rows), dim3(kCombineWarps * 32), 0, st, a);
+    // An item has workers / items parts where its sequence is as long as the others, and up to all of them where it is the only long one.
+    // With few items there are few rows as well, and a block of 16 warps for each costs nothing: two of 65537 tokens, 296 parts an item,
+    // XXX us by four warps, XXX by sixteen; 64 of 8192, five parts, XXX and XXX.
+    const bool wide = (long long)a.B * g.n_kv * a.col_tiles * 16 <= a.workers;
+    auto combine = g.head_dim == 64   ? (wide ? paged_combine_kernel<64, 16> : paged_combine_kernel<64, 4>)
+                   : g.head_dim == 96 ? (wide ? paged_combine_kernel<96, 16> : paged_combine_kernel<96, 4>)
+                                      : (wide ? paged_combine_kernel<128, 16> : paged_combine_kernel<128, 4>);
+    const size_t smem = (size_t)kWarps * (g.head_dim == 64 ? Ring<64>::kBytes : g.head_dim == 96 ? Ring<96>::kBytes : Ring<128>::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = launch_kernel(false, kernel, dim3((unsigned)(a.workers / kWarps)), dim3(kWarps * 32), smem, st, a);
+    if (e == cudaSuccess) e = launch_kernel(true, combine, dim3((unsigned)rows), dim3((wide ? 16 : 4) * 32), 0, st, a);
     if (e != cudaSuccess) {
         set_cuda_error(e, "paged attention launch");
         return FLASHMHF_ERR_CUDA;
