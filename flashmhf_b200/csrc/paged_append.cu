@@ -1,7 +1,7 @@
 // New tokens of packed sequences: rotary embedding of queries and keys, and keys and values into the pages of the 8-bit cache.
 //
 // One launch does all of it: its blocks are split between "pages" (one page, key/value head and K or V each: the scale of a page
-// depends on all of its new rows, so one block sees them all) and "queries".  A page's new rows stay in registers between the
+// depends on all of its new rows, so one block sees them all; of single tokens sixteen to a block) and "queries".  A page's new rows stay in registers between the
 // maximum and the rounding, so everything is read once and written once: bound by HBM for prompts, by latency for single tokens.
 #include "paged.cuh"
 #include "tc_common.cuh"
@@ -123,17 +123,13 @@ __device__ void append_page(const AppendArgs &a, int P, uint32_t *red) {
     constexpr int PAIRS = HD / 16, kMaxPasses = 4;       // eight threads a row; at most 128 rows by 256 threads, or 16 by 128
     const int kv2 = 2 * a.n_kv;
     const int slot = (int)(blockIdx.x / (unsigned)kv2), hk = (int)(blockIdx.x % (unsigned)kv2), head = hk >> 1, which = hk & 1;
-    int b = slot, j = 0;
-    if (a.cu) {
-        int lo = 0, hi = a.B - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (__ldg(a.cu + mid) / P + 2 * mid <= slot) lo = mid;
-            else hi = mid - 1;
-        }
-        b = lo;
-        j = slot - (__ldg(a.cu + b) / P + 2 * b);
+    int b = 0, hi = a.B - 1;
+    while (b < hi) {
+        const int mid = (b + hi + 1) >> 1;
+        if (__ldg(a.cu + mid) / P + 2 * mid <= slot) b = mid;
+        else hi = mid - 1;
     }
+    const int j = slot - (__ldg(a.cu + b) / P + 2 * b);
     const Piece pc = piece_of(a, b);
     if (pc.last <= pc.first || j < 0) return;
     // (64 bits: a length near 2^31 is the caller's mistake, not a wrap-around)
@@ -210,6 +206,61 @@ __device__ void append_page(const AppendArgs &a, int P, uint32_t *red) {
     }
 }
 
+// One token a sequence: eight threads a (sequence, head, K or V).  The page's other rows are touched only where its scale grows.
+template <int HD>
+__device__ void append_token(const AppendArgs &a, int P) {
+    constexpr int PAIRS = HD / 16;
+    const long long it = (long long)blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3);
+    const int sub = threadIdx.x & 7, which = (int)(it & 1), head = (int)((it >> 1) % a.n_kv);
+    const unsigned group = 0xffu << (threadIdx.x & 24);
+    const long long b = (it >> 1) / a.n_kv;
+    if (b >= a.B) return;
+    // (the row is asked for before its place is known)
+    float y1[PAIRS], y2[PAIRS];
+    const __nv_bfloat16 *src = a.x[which] + b * a.x_tok[which] + head * a.x_head[which] + sub * PAIRS;
+    load_bf16<PAIRS>(src, y1);
+    load_bf16<PAIRS>(src + HD / 2, y2);
+    const int pos = __ldg(a.lengths + b);
+    if (pos < 0) return;
+    const int page_no = pos / P, row = pos % P;
+    const int page = page_no < a.max_pages ? __ldg(a.table + b * a.table_stride + page_no) : -1;
+    if (page < 0 || page >= a.num_pages || pos >= a.max_pos) {
+        note_index(a.status, page < 0 || page >= a.num_pages ? kPagedAppendPage : kPagedAppendPosition);
+        return;
+    }
+    float *sp = a.scale[which] + (long long)page * a.n_kv + head;
+    const float old = *sp;
+    if (which == 0) {
+        float c[PAIRS], s[PAIRS];
+        load_f32<PAIRS>(a.cos_t + (long long)pos * (HD / 2) + sub * PAIRS, c);
+        load_f32<PAIRS>(a.sin_t + (long long)pos * (HD / 2) + sub * PAIRS, s);
+        rotate<PAIRS>(y1, y2, c, s);
+        if (a.k_out) {
+            __nv_bfloat16 *dst = a.k_out + (b * a.n_kv + head) * HD + sub * PAIRS;
+            store_bf16<PAIRS>(dst, y1);
+            store_bf16<PAIRS>(dst + HD / 2, y2);
+        }
+    }
+    uint32_t amax = max_finite<PAIRS>(max_finite<PAIRS>(0, y1), y2);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(group, amax, o));
+    const float need = scale_for(amax), now = row > 0 ? fmaxf(old, need) : need, inv = 1.f / now;
+    uint8_t *dst = a.pages[which] + page * a.page_stride + (long long)head * P * HD;
+    __syncwarp(group);                           // all eight have read the scale
+    if (sub == 0 && now != old) *sp = now;
+    store_codes<PAIRS>(dst + row * HD + sub * PAIRS, y1, inv);
+    store_codes<PAIRS>(dst + row * HD + HD / 2 + sub * PAIRS, y2, inv);
+    if (row > 0 && now != old) {
+        const float ratio = old * inv;
+#pragma unroll 4
+        for (int i = sub; i < row * (HD / 16); i += 8) {
+            uint4 *c = reinterpret_cast<uint4 *>(dst) + i;
+            const uint4 v = *c;
+            *c = make_uint4(rescale4(v.x, ratio), rescale4(v.y, ratio), rescale4(v.z, ratio), rescale4(v.w, ratio));
+        }
+    }
+}
+
 // Which sequence a token belongs to (the last b with cu[b] <= t), and its position; -1 where it has none.
 __device__ __forceinline__ long long position_of(const AppendArgs &a, int t) {
     int b = t;
@@ -261,8 +312,9 @@ __device__ void append_queries(const AppendArgs &a) {
 template <int HD>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int P) {
     __shared__ uint32_t red[8];
-    if (blockIdx.x < a.page_blocks) append_page<HD>(a, P, red);
-    else append_queries<HD>(a);
+    if (blockIdx.x >= a.page_blocks) append_queries<HD>(a);
+    else if (a.cu) append_page<HD>(a, P, red);
+    else append_token<HD>(a, P);
 }
 
 }  // namespace
@@ -286,9 +338,8 @@ int paged_append(const flashmhf_paged_append_params &p, const DeviceCtl &ctl, cu
     a.status = ctl.status;
     a.B = p.seq.B; a.max_pages = p.seq.max_pages; a.num_pages = g.num_pages; a.n_kv = g.n_kv;
     a.tokens = p.tokens; a.n_q = p.q ? p.n_q : 0; a.max_pos = p.max_positions;
-    const int P = g.page_size, threads = P * 8 < 256 ? P * 8 : 256;
-    const long long slots = a.cu ? (long long)p.tokens / P + 2ll * a.B : a.B;
-    const long long page_blocks = slots * 2 * a.n_kv;
+    const int P = g.page_size, threads = a.cu ? (P * 8 < 256 ? P * 8 : 256) : 128;
+    const long long page_blocks = a.cu ? ((long long)p.tokens / P + 2ll * a.B) * 2 * a.n_kv : ((long long)a.B * 2 * a.n_kv + 15) / 16;
     const long long groups = a.n_q ? (a.n_q + kHeadsPerThread - 1) / kHeadsPerThread : 0, per_block = threads / 8;
     const long long blocks = page_blocks + ((long long)p.tokens * groups + per_block - 1) / per_block;
     if (blocks > 0x7fffffffll) return FLASHMHF_ERR_BAD_SHAPE;

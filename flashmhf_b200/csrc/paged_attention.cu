@@ -17,6 +17,8 @@
 // largest is between 2^14 and 2^15: exact down to 2^-28 of it.  P is rounded to 11 bits; maxima, sums and O are fp32.
 // Which dims a lane's share of a fragment stands for is free as long as both operands agree, so a lane loads HD / 4 neighbouring codes of a
 // key and HD / 8 of a value, straight into fragments; pairs of tokens that V needs side by side are made by byte permutation.
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc_common.cuh"
 
@@ -135,6 +137,27 @@ __device__ long long units_between(const PagedArgs &a, int first, int last) {
     return warp_sum(n);
 }
 
+// Units dealt out: worker w has first(w) .. first(w + 1) - 1; the first `extra` workers have one more than the others, and every worker has one.
+struct Deal {
+    int workers, extra;
+    long long each;
+    __device__ Deal(long long total, int most) {
+        workers = (int)min((long long)most, total);
+        const long long w = max(workers, 1);
+        each = divide(total, w);
+        extra = (int)(total - each * w);
+    }
+    // 32-bit division where it fits: the 64-bit one is a hundred instructions
+    static __device__ __forceinline__ long long divide(long long a, long long b) {
+        return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+    }
+    __device__ __forceinline__ long long first(int w) const { return w * each + min(w, extra); }
+    __device__ __forceinline__ int owner(long long unit) const {
+        const long long cut = extra * (each + 1);
+        return (int)(unit < cut ? divide(unit, each + 1) : extra + divide(unit - cut, each));
+    }
+};
+
 // What a stage's pages stand for, by its 16 tokens: key scale (NaN: no page), exponent of the value scale (clamped), the rest of that scale.
 struct Granule {
     float ks, ve, vr, pad;
@@ -162,11 +185,10 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
     if (abort_flag) return;
     uint32_t issued = 0, used = 0;      // stages, counted through all of the run
     const int per_seq = a.n_kv * a.col_tiles, P = 1 << a.log_page, rows = a.group * a.n_new;
-    const long long total = units_between(a, 0, a.B) * per_seq;
-    const int workers = (int)min((long long)a.workers, total);       // each has a unit at least
-    if (worker >= workers) return;
-    long long u = total * worker / workers;
-    const long long u_end = total * (worker + 1) / workers, u_first = u;
+    const Deal deal(units_between(a, 0, a.B) * per_seq, a.workers);
+    if (worker >= deal.workers) return;
+    long long u = deal.first(worker);
+    const long long u_end = deal.first(worker + 1), u_first = u;
 
     // the sequence that unit u belongs to, and where its units begin
     int b = 0;
@@ -196,28 +218,97 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
             len = length_of(a, ++b);
             n_units = units_of(len);
         }
-        const int item = (int)((u - base) / n_units), head = item / a.col_tiles, col0 = (item % a.col_tiles) * kCols;
+        const int item = (int)Deal::divide(u - base, n_units), head = item / a.col_tiles, col0 = (item % a.col_tiles) * kCols;
         const long long begin = base + item * n_units, end = begin + n_units, stop = min(end, u_end);
         const int tok0 = (int)(u - begin) * kUnit, tok1 = (int)min((long long)len, (stop - begin) * kUnit);
 
-        // queries: column g of the tile, dims HD / 4 * t on
+        // tokens that the lane's columns see
+        int see[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) see[i] = len - (a.n_new - 1 - min(rows - 1, col0 + 2 * t + i) / a.group);
+        const int all = len - (a.n_new - 1);
+
+        // queries: column g of the tile, dims HD / 4 * t on (asked for here, put into fragments when the codes are on their way)
+        uint32_t raw_q[HD / 8] = {};
+        if (col0 + g < rows) {
+            const int r = col0 + g;
+            load_words<HD / 8>(reinterpret_cast<const uint8_t *>(a.q + b * a.q_stride[0] + (r / a.group) * a.q_stride[1] +
+                                                                 (head * a.group + r % a.group) * a.q_stride[2] + t * (HD / 4)), raw_q);
+        }
+
+        // pages: lane i knows page first_page + i and its scales, and those of the 32 after
+        const int32_t *table = a.table + b * a.table_stride;
+        const int last_page = (tok1 - 1) >> a.log_page;
+        int page_base = tok0 >> a.log_page;
+        int id, id2;
+        float ks, vs, ks2, vs2;
+        auto pages = [&](int first, int &pid, float &k, float &v) {
+            pid = first + lane <= last_page ? __ldg(table + first + lane) : -1;
+            if (first + lane <= last_page && (pid < 0 || pid >= a.num_pages)) {
+                note_index(a.status, kPagedAttnPage);
+                pid = -1;
+            }
+            const long long at = (long long)max(pid, 0) * a.n_kv + head;      // (of no page: any scale)
+            k = __ldg(a.k_scale + at);
+            v = __ldg(a.v_scale + at);
+        };
+        pages(page_base, id, ks, vs);
+        float o[MT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        // Copies of the stage of tokens from `tok` on.  The warp has read what was there (it meets before each call).
+        auto load = [&](int tok) {
+            const uint32_t st = issued++ % NS, dst = ring_at + st * R::kStage, bar = bar_at + 8 * st;
+            const int n = min(R::kTokens, (tok1 - tok + 15) & ~15), step = min(P, n);       // whole 16s: rows of a page exist, used or not
+            int pid[NG], at_lane[NG] = {};
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                pid[i] = -1;
+                if (i * 16 < n) {
+                    int pi = ((tok + i * 16) >> a.log_page) - page_base;
+                    if (pi >= 32) {
+                        id = id2; ks = ks2; vs = vs2;       // (never between the 16s of a stage: pages of 16 come in fours)
+                        page_base += 32;
+                        pi -= 32;
+                        pages(page_base + 32, id2, ks2, vs2);
+                    }
+                    at_lane[i] = pi;
+                    pid[i] = __shfl_sync(0xffffffffu, id, pi);
+                    if (pid[i] >= 0) bytes += 2 * 16 * HD;
+                }
+            }
+            if (lane == 0) {
+                if (bytes) mbar_arrive_expect_tx(bar, bytes);
+                else mbar_arrive(bar);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    // (a page of 32 or more holds the stage: one copy of each kind)
+                    if (i * 16 >= n || pid[i] < 0 || (i > 0 && step > 16)) continue;
+                    const long long at = (long long)pid[i] * a.page_stride + ((long long)head * P + ((tok + i * 16) & (P - 1))) * HD;
+                    const uint32_t size = (step > 16 ? n : 16) * HD;
+                    bulk_load(dst + i * 16 * HD, a.k + at, size, bar);
+                    bulk_load(dst + R::kHalf + i * 16 * HD, a.v + at, size, bar);
+                }
+            }
+            // (after the copies: they do not wait for the scales)
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const float k = __shfl_sync(0xffffffffu, ks, at_lane[i]), v = __shfl_sync(0xffffffffu, vs, at_lane[i]);
+                const int e = min(max((int)(__float_as_uint(v) >> 23 & 255) - 127, -kMaxExp), kMaxExp);
+                if (lane == 0) granules[warp][st][i] = Granule{pid[i] < 0 ? NAN : k, (float)e, v * __uint_as_float((uint32_t)(127 - e) << 23), 0.f};
+            }
+        };
+        for (int i = 0; i < NS; ++i)
+            if (tok0 + i * R::kTokens < tok1) load(tok0 + i * R::kTokens);
+        __syncwarp();
+        pages(page_base + 32, id2, ks2, vs2);      // (a few stages do not reach them)
         uint32_t qf[KK][2];
         float fac[2];                                    // what scores of columns 2t, 2t + 1 are multiplied by
         {
-            const int r = col0 + g;
             float x[HD / 4], top = 0.f;
-            if (r < rows) {
-                const __nv_bfloat16 *q = a.q + b * a.q_stride[0] + (r / a.group) * a.q_stride[1] + (head * a.group + r % a.group) * a.q_stride[2] + t * (HD / 4);
-                uint32_t w[HD / 8];
-                load_words<HD / 8>(reinterpret_cast<const uint8_t *>(q), w);
 #pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    x[2 * i] = __uint_as_float(w[i] << 16);
-                    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < HD / 4; ++i) x[i] = 0.f;
+            for (int i = 0; i < HD / 8; ++i) {
+                x[2 * i] = __uint_as_float(raw_q[i] << 16);
+                x[2 * i + 1] = __uint_as_float(raw_q[i] & 0xffff0000u);
             }
 #pragma unroll
             for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(x[i]));
@@ -234,79 +325,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
             fac[0] = a.c * __shfl_sync(0xffffffffu, down, 8 * t);
             fac[1] = a.c * __shfl_sync(0xffffffffu, down, 8 * t + 4);
         }
-        // tokens that the lane's columns see
-        int see[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) see[i] = len - (a.n_new - 1 - min(rows - 1, col0 + 2 * t + i) / a.group);
-        const int all = len - (a.n_new - 1);
-
-        // pages: lane i knows page first_page + i and its scales, and those of the 32 after
-        const int32_t *table = a.table + b * a.table_stride;
-        const int last_page = (tok1 - 1) >> a.log_page;
-        int page_base = tok0 >> a.log_page;
-        int id, id2;
-        float ks, ve, vr, ks2, ve2, vr2;
-        auto pages = [&](int first, int &pid, float &k, float &e, float &r) {
-            pid = first + lane <= last_page ? __ldg(table + first + lane) : -1;
-            if (first + lane <= last_page && (pid < 0 || pid >= a.num_pages)) {
-                note_index(a.status, kPagedAttnPage);
-                pid = -1;
-            }
-            k = e = 0.f;
-            r = 1.f;
-            if (pid >= 0) {
-                k = __ldg(a.k_scale + (long long)pid * a.n_kv + head);
-                const float v = __ldg(a.v_scale + (long long)pid * a.n_kv + head);
-                const int n = min(max((int)(__float_as_uint(v) >> 23 & 255) - 127, -kMaxExp), kMaxExp);
-                e = (float)n;
-                r = v * __uint_as_float((uint32_t)(127 - n) << 23);
-            }
-        };
-        pages(page_base, id, ks, ve, vr);
-        pages(page_base + 32, id2, ks2, ve2, vr2);
-
-        float o[MT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        // Copies of the stage of tokens from `tok` on.  The warp has read what was there (it meets before each call).
-        auto load = [&](int tok) {
-            const uint32_t st = issued++ % NS, dst = ring_at + st * R::kStage, bar = bar_at + 8 * st;
-            const int n = min(R::kTokens, (tok1 - tok + 15) & ~15), step = min(P, n);       // whole 16s: rows of a page exist, used or not
-            int pid[NG];
-            uint32_t bytes = 0;
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                pid[i] = -1;
-                if (i * 16 < n) {
-                    int pi = ((tok + i * 16) >> a.log_page) - page_base;
-                    if (pi >= 32) {
-                        id = id2; ks = ks2; ve = ve2; vr = vr2;
-                        page_base += 32;
-                        pi -= 32;
-                        pages(page_base + 32, id2, ks2, ve2, vr2);
-                    }
-                    pid[i] = __shfl_sync(0xffffffffu, id, pi);
-                    Granule x;
-                    x.ks = __shfl_sync(0xffffffffu, ks, pi);
-                    x.ve = __shfl_sync(0xffffffffu, ve, pi);
-                    x.vr = __shfl_sync(0xffffffffu, vr, pi);
-                    if (pid[i] < 0) x.ks = NAN;
-                    else bytes += 2 * 16 * HD;
-                    if (lane == 0) granules[warp][st][i] = x;
-                }
-            }
-            if (lane == 0) {
-                if (bytes) mbar_arrive_expect_tx(bar, bytes);
-                else mbar_arrive(bar);
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    // (a page of 32 or more holds the stage: one copy of each kind)
-                    if (i * 16 >= n || pid[i] < 0 || (i > 0 && step > 16)) continue;
-                    const long long at = (long long)pid[i] * a.page_stride + ((long long)head * P + ((tok + i * 16) & (P - 1))) * HD;
-                    const uint32_t size = (step > 16 ? n : 16) * HD;
-                    bulk_load(dst + i * 16 * HD, a.k + at, size, bar);
-                    bulk_load(dst + R::kHalf + i * 16 * HD, a.v + at, size, bar);
-                }
-            }
-        };
         auto compute = [&](int tok, const uint8_t *keys, const Granule st) {
             const bool none = st.ks != st.ks;
             const int left = none ? 0 : tok1 - tok;       // tokens of the 16 that are there; what lies behind them may be anything
@@ -372,8 +390,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
                 }
             }
         };
-        for (int i = 0; i < NS; ++i)
-            if (tok0 + i * R::kTokens < tok1) load(tok0 + i * R::kTokens);
         for (int tok = tok0; tok < tok1; tok += R::kTokens, ++used) {
             const uint32_t st = used % NS;
             if (!__all_sync(0xffffffffu, mbar_wait(bar_at + 8 * st, (used / NS) & 1, ctl, kKernelPaged * 100 + 1))) {
@@ -421,9 +437,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
             }
         }
         if (stop == end && lane == 0) {
-            // the worker of unit x is the last w with floor(w total / workers) <= x
-            const int w0 = (int)(((begin + 1) * workers - 1) / total);
-            a.shared_by[(long long)b * per_seq + item] = make_int4(w0, worker, total * w0 / workers < begin ? 1 : 0, 0);
+            const int w0 = u_first <= begin ? worker : deal.owner(begin);
+            a.shared_by[(long long)b * per_seq + item] = make_int4(w0, worker, deal.first(w0) < begin ? 1 : 0, 0);
         }
         u = stop;
     }
@@ -443,33 +458,55 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
     griddep_wait();        // launched early, behind the kernel whose parts it adds
     const int4 by = empty ? make_int4(0, 0, 0, 0) : a.shared_by[((long long)b * a.n_kv + head) * a.col_tiles + r / kCols];
     if (!empty && by.x == by.y) return;
-    auto at = [&](int w) { return ((long long)w * 2 + (w == by.x ? by.z : 0)) * kCols + col; };
-    float m = -INFINITY, l = 0.f, o[N] = {};
+    float m = -INFINITY, l = 0.f;
     if (!empty) {
-        for (int w = by.x + threadIdx.x; w <= by.y; w += kCombineWarps * 32) m = fmaxf(m, a.ml[at(w)].x);
+        // each warp its own maximum, some parts in flight
+        constexpr int U = kCombineWarps == 4 ? 2 : 8;
+        float o[N] = {};
+        for (int w0 = by.x + warp; w0 <= by.y; w0 += U * kCombineWarps) {
+            float2 ml[U];
+            float v[U][N] = {};
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        if (lane == 0) top[warp] = m;
-        __syncthreads();
+            for (int i = 0; i < U; ++i) {
+                const int w = w0 + i * kCombineWarps;
+                ml[i] = make_float2(-INFINITY, 0.f);
+                if (w <= by.y) {
+                    const long long at = ((long long)w * 2 + (w == by.x ? by.z : 0)) * kCols + col;
+                    ml[i] = a.ml[at];
 #pragma unroll
-        for (int i = 0; i < kCombineWarps; ++i) m = fmaxf(m, top[i]);
-        const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-        for (int w = by.x + warp; w <= by.y; w += kCombineWarps) {
-            const long long i = at(w);
-            const float2 ml = a.ml[i];
-            const float f = ex2(ml.x - ref);
-            l = fmaf(ml.y, f, l);
+                    for (int x = 0; x < N; ++x) v[i][x] = a.part[at * HD + x * 32 + lane];
+                }
+            }
+            float now = m;
 #pragma unroll
-            for (int x = 0; x < N; ++x) o[x] = fmaf(a.part[i * HD + x * 32 + lane], f, o[x]);
+            for (int i = 0; i < U; ++i) now = fmaxf(now, ml[i].x);
+            const float ref = now == -INFINITY ? 0.f : now, keep = ex2(m - ref);
+            m = now;
+            l *= keep;
+#pragma unroll
+            for (int x = 0; x < N; ++x) o[x] *= keep;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const float f = ex2(ml[i].x - ref);
+                l = fmaf(ml[i].y, f, l);
+#pragma unroll
+                for (int x = 0; x < N; ++x) o[x] = fmaf(v[i][x], f, o[x]);
+            }
         }
 #pragma unroll
         for (int x = 0; x < N; ++x) sum[warp][x * 32 + lane] = o[x];
-        if (lane == 0) weights[warp] = l;
+        if (lane == 0) {
+            top[warp] = m;
+            weights[warp] = l;
+        }
         __syncthreads();
+        m = top[0];
+#pragma unroll
+        for (int i = 1; i < kCombineWarps; ++i) m = fmaxf(m, top[i]);
+        const float ref = m == -INFINITY ? 0.f : m;
         l = 0.f;
 #pragma unroll
-        for (int i = 0; i < kCombineWarps; ++i) l += weights[i];
+        for (int i = 0; i < kCombineWarps; ++i) l = fmaf(weights[i], ex2(top[i] - ref), l);
     }
     __nv_bfloat16 *dst = a.o + b * a.o_stride[0] + n * a.o_stride[1] + h * a.o_stride[2];
     const float f = l == 0.f ? 0.f : 1.f / l;
@@ -477,7 +514,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
         float y = 0.f;
         if (!empty)
 #pragma unroll
-            for (int i = 0; i < kCombineWarps; ++i) y += sum[i][d];
+            for (int i = 0; i < kCombineWarps; ++i) y = fmaf(sum[i][d], ex2(top[i] - (m == -INFINITY ? 0.f : m)), y);
         dst[d] = __float2bfloat16(l == 0.f ? 0.f : y * f);
     }
     if (a.lse && threadIdx.x == 0) a.lse[((long long)b * a.n_new + n) * a.n_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -524,7 +561,13 @@ int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &c
                    : g.head_dim == 96 ? (wide ? paged_combine_kernel<96, 16> : paged_combine_kernel<96, 4>)
                                       : (wide ? paged_combine_kernel<128, 16> : paged_combine_kernel<128, 4>);
     const size_t smem = (size_t)kWarps * (g.head_dim == 64 ? Ring<64>::kBytes : g.head_dim == 96 ? Ring<96>::kBytes : Ring<128>::kBytes);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaSuccess;
+    static std::atomic<bool> done[3][64];      // the attribute is per kernel and device
+    std::atomic<bool> &set = done[g.head_dim / 32 - 2][ctl.device];
+    if (!set.load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        set.store(e == cudaSuccess, std::memory_order_release);
+    }
     if (e == cudaSuccess) e = launch_kernel(false, kernel, dim3((unsigned)(a.workers / kWarps)), dim3(kWarps * 32), smem, st, a);
     if (e == cudaSuccess) e = launch_kernel(true, combine, dim3((unsigned)rows), dim3((wide ? 16 : 4) * 32), 0, st, a);
     if (e != cudaSuccess) {

@@ -18,6 +18,8 @@
 //
 // Warp roles: 0-3 and 4-7 softmax of the two tiles (warp % 4 = TMEM lane quarter = 32 rows), 8 work items and TMA, 9 and 10 MMA issuers of
 // the two tiles.  Warp 9 also clears the rows of V behind the end of a sequence (a weight of 0 does not undo a NaN of the next one).
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc_common.cuh"
 #include "tensormap.cuh"
@@ -459,7 +461,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 }
 
 template <int HD>
-int launch_prompt(const flashmhf_prompt_attention_params &p, const PromptArgs &a, int num_sms, cudaStream_t st, int *n_launch) {
+int launch_prompt(const flashmhf_prompt_attention_params &p, const PromptArgs &a, int num_sms, int device, cudaStream_t st, int *n_launch) {
     CUtensorMap q, k, v;
     auto map = [&](CUtensorMap *m, const void *ptr, const int64_t *stride, int heads, int tokens) {
         if (tokens == 0) heads = tokens = 1;      // no keys at all: nothing is read through the map
@@ -473,7 +475,12 @@ int launch_prompt(const flashmhf_prompt_attention_params &p, const PromptArgs &a
     if (rc == FLASHMHF_OK) rc = map(&v, p.v, p.v_stride, p.n_kv, p.tokens_k);
     if (rc != FLASHMHF_OK) return rc;
     const size_t smem = PromptCfg<HD>::kTotal;
-    cudaError_t e = cudaFuncSetAttribute(prompt_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaSuccess;
+    static std::atomic<bool> done[64];      // the attribute is per kernel and device
+    if (!done[device].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(prompt_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        done[device].store(e == cudaSuccess, std::memory_order_release);
+    }
     if (e == cudaSuccess)
         e = launch_kernel(false, prompt_attention_kernel<HD>, dim3((unsigned)(a.n_items < num_sms ? a.n_items : num_sms)), dim3(kThreads), smem, st, q, k, v, a);
     if (e != cudaSuccess) {
@@ -501,9 +508,9 @@ int prompt_attention(const flashmhf_prompt_attention_params &p, const DeviceCtl 
     a.c = c > 1e-30f ? c : 1e-30f;
     a.wait = wait_args(&ctl);
     switch (p.head_dim) {
-        case 64: return launch_prompt<64>(p, a, ctl.num_sms, st, n_launch);
-        case 96: return launch_prompt<96>(p, a, ctl.num_sms, st, n_launch);
-        default: return launch_prompt<128>(p, a, ctl.num_sms, st, n_launch);
+        case 64: return launch_prompt<64>(p, a, ctl.num_sms, ctl.device, st, n_launch);
+        case 96: return launch_prompt<96>(p, a, ctl.num_sms, ctl.device, st, n_launch);
+        default: return launch_prompt<128>(p, a, ctl.num_sms, ctl.device, st, n_launch);
     }
 }
 
