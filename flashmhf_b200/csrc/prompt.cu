@@ -31,6 +31,7 @@ constexpr int kRows = 128, kKeys = 128, kItemRows = 2 * kRows;
 constexpr int kThreads = 11 * 32;   // 184 registers a thread: a softmax thread holds a row of S, 128 of them
 constexpr uint32_t kTileChunk = 128 * 128;        // 128 rows of 64 columns
 constexpr int kKernelPrompt = 6;                  // status codes 601..
+constexpr int kLag = 8;
 constexpr float kLazy = 8.f;                      // how far (in powers of two) the maximum may be exceeded before O is scaled again
 
 template <int HD>
@@ -47,7 +48,7 @@ struct PromptCfg {
 // OFULL[g]: the last of an item; OFREE[g]: O has been read out; ITEM*: the ring of work items.
 enum { PB_QFULL = 0, PB_QEMPTY = 1, PB_SFULL = 2, PB_SFREE = 4, PB_PFULL = 6, PB_PVDONE = 8, PB_OFULL = 10, PB_OFREE = 12, PB_ITEMFULL = 14,
        PB_ITEMEMPTY = 16, PB_KFULL = 18, PB_KEMPTY = 22, PB_VFULL = 26, PB_VEMPTY = 30, PB_VRAW = 34, PB_COUNT = 38 };
-static_assert(PB_COUNT * 8 + 16 + 2 * 48 <= 512, "control area");
+static_assert(PB_COUNT * 8 + 16 + 2 * 48 + 32 <= 512, "control area");
 
 struct PromptItem {
     int q0, lq;          // first row of the item in the packed rows; rows of the sequence from there on
@@ -146,6 +147,22 @@ __device__ __forceinline__ bool thread_wait(uint32_t bar, uint32_t parity, const
     return true;
 }
 
+// Turns at the special function unit of a quarter of the SM, which warps w and w + 4 share.  Left to themselves the two tiles fall into step:
+// both take their exponentials at half speed and then wait for the tensor core together.  0: elsewhere, 1: wants it, 2: has it; of two
+// that come together the first tile goes first.  A matter of speed only: whoever has waited 2000 clk goes ahead.
+struct Turn {
+    volatile int *mine, *other;
+    int stop_at;                      // state of the other that this one waits for to end
+    __device__ Turn(volatile int *turns, int warp) : mine(turns + warp), other(turns + (warp ^ 4)), stop_at(warp < 4 ? 2 : 1) {}
+    __device__ __forceinline__ void take() {
+        *mine = 1;
+        const long long t0 = clock64();
+        while (*other >= stop_at && clock64() - t0 < 2000) {}
+        *mine = 2;
+    }
+    __device__ __forceinline__ void give() { *mine = 0; }
+};
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -160,6 +177,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gbase + L::kOffBar + PB_COUNT * 8);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(gbase + L::kOffBar + PB_COUNT * 8 + 4);
     volatile int *items = reinterpret_cast<volatile int *>(gbase + L::kOffBar + PB_COUNT * 8 + 16);   // two of 12 words
+    volatile int *turns = items + 24;                                                                 // eight: see Turn
     auto bar = [&](int i) { return sBar + 8u * i; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtl ctl{abort_flag, args.wait};
@@ -179,6 +197,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             mbar_init(bar(PB_ITEMFULL + g), 1);
             mbar_init(bar(PB_ITEMEMPTY + g), 10);   // every warp but the one that fills it
         }
+        for (int i = 0; i < 8; ++i) turns[i] = 0;
         for (int i = 0; i < NS; ++i) {
             mbar_init(bar(PB_KFULL + i), 1);
             mbar_init(bar(PB_KEMPTY + i), 2);
@@ -329,6 +348,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t tS = lanes + t * 128, tP = lanes + L::kColP + t * L::kPStride, tO = lanes + L::kColO + t * L::kOStride;
         const float c = args.c;
+        Turn turn(turns, warp);
         PromptItem w;
         uint32_t steps = 0;
         int outs = 0;
@@ -390,22 +410,28 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     if (!warp_wait(bar(PB_PVDONE + t), (steps - 1) & 1, ctl, W + 17)) { ok = false; break; }
                     tc_fence_after();
                 }
+                turn.take();
+                // Exponents first, then exponentials with their sums and roundings eight behind: in program order nothing waits for the
+                // result just asked for.
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {      // 64 columns at a time: P takes the registers of S as it goes
-                  uint32_t p[32];
+                for (int i = 0; i < 128; i += 2) f2_unpack(f2_fma(f2_pack(s[i], s[i + 1]), c2, mc2), s[i], s[i + 1]);
+                uint32_t p[32];
 #pragma unroll
-                  for (int i = 64 * h; i < 64 * h + 64; i += 4) {
-                    float e0, e1, e2, e3;
-                    f2_unpack(f2_fma(f2_pack(s[i], s[i + 1]), c2, mc2), e0, e1);
-                    f2_unpack(f2_fma(f2_pack(s[i + 2], s[i + 3]), c2, mc2), e2, e3);
-                    e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
-                    sum0 = f2_add(sum0, f2_pack(e0, e1));
-                    sum1 = f2_add(sum1, f2_pack(e2, e3));
-                    p[(i - 64 * h) / 2] = pack_bf16(e0, e1);
-                    p[(i - 64 * h) / 2 + 1] = pack_bf16(e2, e3);
-                  }
-                  tmem_st32(tP + 32 * h, p);
+                for (int i = 0; i < 128 + kLag; i += 4) {
+                    if (i < 128) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) s[i + k] = ex2(s[i + k]);
+                    }
+                    if (i >= kLag) {
+                        const int x = i - kLag;
+                        sum0 = f2_add(sum0, f2_pack(s[x], s[x + 1]));
+                        sum1 = f2_add(sum1, f2_pack(s[x + 2], s[x + 3]));
+                        p[(x & 63) / 2] = pack_bf16(s[x], s[x + 1]);
+                        p[(x & 63) / 2 + 1] = pack_bf16(s[x + 2], s[x + 3]);
+                        if ((x & 63) == 60) tmem_st32(tP + (x >> 6) * 32, p);
+                    }
                 }
+                turn.give();
                 float a0, a1;
                 f2_unpack(f2_add(sum0, sum1), a0, a1);
                 l += a0 + a1;
