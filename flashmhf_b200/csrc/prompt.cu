@@ -13,14 +13,16 @@
 // The maximum is lazy: O is multiplied by 2^(c m_old - c m_new) only where a new maximum is more than 2^8 above the one in use (P is then
 // at most 256, and P, its sum and O are all in one scale), so that almost no step touches O.
 //
-// A product never writes tensor memory that another one may still read because of the order of issue alone (that order is promised for products
-// of one accumulator and shape): S of step s + 2 waits until the product that reads P of step s is done.
+// No product writes tensor memory that another one may still be reading on the strength of the order of issue alone (that order is promised for
+// products of one accumulator and shape).  A head of 64 leaves room for P beside S; with heads of 96 and 128 P lies over S, and S of step s + 2
+// waits until the product that reads P of step s is done.
 //
 // Work items are handed out by the hardware: the grid has a block for each, a resident block takes over one that has not started
 // (clusterlaunchcontrol) while it works on its own.
 //
 // Warp roles: 0-15 softmax (tile of rows = warp / 8, parity of the steps = warp / 4 % 2, TMEM lane quarter = warp % 4), 16 work items and TMA, 17
-// and 18 MMA issuers of the two tiles, 19 clears the rows of V behind the end of a sequence (a weight of 0 does not undo a NaN of the next one).
+// issues S of both tiles, 18 and 19 O += P V of one each; 18 also clears the rows of V behind the end of a sequence (a weight of 0 does not undo a
+// NaN of the next one).
 #include <atomic>
 
 #include "paged.cuh"
@@ -33,8 +35,8 @@ namespace {
 constexpr int kRows = 128, kItemRows = 2 * kRows, kKeys = 64;
 constexpr int kSoftmaxWarps = 16, kThreads = (kSoftmaxWarps + 4) * 32;
 constexpr int kKernelPrompt = 6;                  // status codes 601..
-constexpr float kLazy = 8.f;                      // how far (in powers of two) the maximum may be exceeded before O is scaled again
-constexpr int kLag = 8, kByPolynomial = 1;        // of each eight exponentials, pairs that the FMA pipe computes
+constexpr float kLazy = 65536.f;                  // the sum of a row's weights of a step above which its reference is set anew
+constexpr int kLag = 8;
 constexpr int kMaxStages = 8;
 
 template <int HD>
@@ -45,15 +47,16 @@ struct PromptCfg {
     static constexpr uint32_t kOffQ = 0, kOffK = kQBufs * 2 * kQTile, kOffV = kOffK + kStages * kTile;
     static constexpr uint32_t kOffMsg = kOffV + kStages * kTile, kOffEnd = kOffMsg + 4 * kRows * 4;   // [tile][parity][row]: maxima; maxima and sums (of two items)
     static constexpr uint32_t kOffBar = kOffEnd + 2 * 4 * kRows * 8, kTotal = kOffBar + 1024 + 1024;
-    // tensor memory: two buffers for S (and P over it) of either tile of rows, and O of both
-    static constexpr uint32_t kColO = 4 * kKeys, kOStride = HD == 64 ? 64 : 128;
+    // tensor memory: two buffers for S of either tile of rows, O of both, and P: over S, or by itself where there is room
+    static constexpr bool kOverlay = HD != 64;
+    static constexpr uint32_t kColP = kOverlay ? 0 : 256, kPStride = kOverlay ? kKeys : kKeys / 2, kColO = kOverlay ? 256 : 384, kOStride = HD == 64 ? 64 : 128;
 };
 
-// SFULL: S computed into a buffer; PFULL: P written over it, O scaled if need be; PVDONE: the product that read P is done (tile t, buffer b:
-// + 2 t + b); OFULL: the last one of an item; OFREE: O has been read out (+ t); MSG: the maximum that a step was taken with (tile t, quarter q,
+// SFULL: S computed into a buffer; SFREE: it is in registers; PFULL: P written, O scaled if need be; PVDONE: the product that read P is done (tile
+// t, buffer b: + 2 t + b); OFULL: the last one of an item; OFREE: O has been read out (+ t); MSG: the maximum that a step was taken with (tile t, quarter q,
 // steps of parity b: + 8 t + 2 q + b); ITEM*: the ring of work items; NEXT: the answer to a request for one.
 enum { PB_QFULL = 0, PB_QEMPTY = 2, PB_SFULL = 4, PB_PFULL = 8, PB_PVDONE = 12, PB_OFULL = 16, PB_OFREE = 18, PB_ITEMFULL = 20, PB_ITEMEMPTY = 22,
-       PB_NEXT = 24, PB_MSG = 25, PB_KFULL = 41, PB_KEMPTY = PB_KFULL + kMaxStages, PB_VFULL = PB_KEMPTY + kMaxStages,
+       PB_NEXT = 24, PB_MSG = 25, PB_SFREE = 41, PB_KFULL = 45, PB_KEMPTY = PB_KFULL + kMaxStages, PB_VFULL = PB_KEMPTY + kMaxStages,
        PB_VEMPTY = PB_VFULL + kMaxStages, PB_VRAW = PB_VEMPTY + kMaxStages, PB_COUNT = PB_VRAW + kMaxStages };
 constexpr uint32_t kOffNext = (PB_COUNT * 8 + 15) / 16 * 16, kOffItems = kOffNext + 16, kOffCtl = kOffItems + 2 * 48;
 static_assert(kOffCtl + 8 <= 1024, "control area");
@@ -194,13 +197,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     auto bar = [&](int i) { return sBar + 8u * i; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtl ctl{abort_flag, args.wait};
-    constexpr int W = kKernelPrompt * 100, kLoad = kSoftmaxWarps, kIssue = kLoad + 1, kEnds = kLoad + 3;
+    constexpr int W = kKernelPrompt * 100, kLoad = kSoftmaxWarps, kIssue = kLoad + 1;
 
     if (threadIdx.x == 0) {
         *abort_flag = launch_aborted(args.wait);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(PB_QFULL + i), 1);
-            mbar_init(bar(PB_QEMPTY + i), 2);
+            mbar_init(bar(PB_QEMPTY + i), 1);
             mbar_init(bar(PB_OFULL + i), 1);
             mbar_init(bar(PB_OFREE + i), 8);
             mbar_init(bar(PB_ITEMFULL + i), 1);
@@ -209,13 +212,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         for (int i = 0; i < 4; ++i) {
             mbar_init(bar(PB_SFULL + i), 1);
             mbar_init(bar(PB_PFULL + i), 4);
+            mbar_init(bar(PB_SFREE + i), 4);
             mbar_init(bar(PB_PVDONE + i), 1);
         }
         for (int i = 0; i < 16; ++i) mbar_init(bar(PB_MSG + i), 1);
         mbar_init(bar(PB_NEXT), 1);
         for (int i = 0; i < NS; ++i) {
             mbar_init(bar(PB_KFULL + i), 1);
-            mbar_init(bar(PB_KEMPTY + i), 2);
+            mbar_init(bar(PB_KEMPTY + i), 1);
             mbar_init(bar(PB_VFULL + i), 1);
             mbar_init(bar(PB_VEMPTY + i), 2);
             mbar_init(bar(PB_VRAW + i), 1);
@@ -310,97 +314,111 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     index = got ? (int)next : -1;
                 }
             }
-        } else if (warp == kEnds) {
-            // -------------------------------------------------------------- V behind the end of a sequence
-            PromptItem w;
-            uint32_t g = 0, seen = 0;      // tiles of keys so far; parities of the stages' raw barriers, which only these tiles use
-            for (int seq = 0; next_item(seq, w); ++seq) {
-                const int n = max(w.n0, w.n1);
-                if (n * kKeys > w.lk) {
-                    const uint32_t st = (g + n - 1) % NS;
-                    if (!warp_wait(bar(PB_VRAW + st), seen >> st & 1, ctl, W + 7)) break;
-                    seen ^= 1u << st;
-                    for (int i = (w.lk - (n - 1) * kKeys) * 8 + lane; i < kKeys * 8; i += 32)
+        } else if (warp == kIssue) {
+            // -------------------------------------------------------------- S of both tiles, whichever can go on
+            if (lane == 0) {
+                constexpr uint32_t idesc = umma_idesc(kRows, kKeys, false, false);
+                const uint64_t dQ0 = desc_kmajor(sQ), dK0 = desc_kmajor(sK);
+                PromptItem w;
+                uint32_t g = 0, steps[2] = {0, 0};      // tiles of keys so far, of all items; those that the tiles of rows needed
+                int n_q = 0;
+                bool ok = true;
+                for (int seq = 0; ok; ++seq) {
+                    if (!thread_wait(bar(PB_ITEMFULL + (seq & 1)), (seq >> 1) & 1, ctl, W + 8)) break;
+                    read_item(seq, w);
+                    mbar_arrive(bar(PB_ITEMEMPTY + (seq & 1)));
+                    if (w.head < 0) break;
+                    const int n = max(w.n0, w.n1), need[2] = {w.n0, w.n1};
+                    if (n == 0) continue;
+                    const int qb = n_q % NQ;
+                    if (!thread_wait(bar(PB_QFULL + qb), (n_q / NQ) & 1, ctl, W + 9)) break;
+                    ++n_q;
+                    int next[2] = {0, 0}, there = 0, back = 0;      // S issued; tiles of keys that have come, that were given back
+                    long long t0 = 0;
+                    while (back < n) {
+                        bool went = false;
+                        if (there < n && there <= max(next[0], next[1])) {
+                            const uint32_t x = g + there;
+                            if (mbar_test(bar(PB_KFULL + x % NS), (x / NS) & 1)) {
+                                ++there;
+                                went = true;
+                            }
+                        }
 #pragma unroll
-                        for (int c = 0; c < L::kChunks; ++c) st_shared_v4(sV + st * L::kTile + c * L::kKChunk + i * 16, 0, 0, 0, 0);
-                    fence_async_smem();
-                    warp_arrive(bar(PB_VFULL + st));
-                }
-                g += n;
-            }
-        } else if (lane == 0) {
-            // -------------------------------------------------------------- MMA issuers, one a tile of rows
-            // Two streams, each in its own order: S, which needs its keys and its buffer, and O += P V, which needs P.  Whichever can go on does.
-            const int t = warp - kIssue;
-            constexpr uint32_t idesc1 = umma_idesc(kRows, kKeys, false, false), idesc2 = umma_idesc(kRows, HD, false, true);
-            const uint64_t dQ0 = desc_kmajor(sQ + t * L::kQTile), dK0 = desc_kmajor(sK), dV0 = desc_mnmajor(sV, L::kKChunk);
-            const uint32_t tO = tmem + L::kColO + t * L::kOStride;
-            PromptItem w;
-            uint32_t g = 0, steps = 0;      // tiles of keys so far, of all items; those of this issuer's rows
-            int n_q = 0, outs = 0;
-            bool ok = true;
-            for (int seq = 0; ok; ++seq) {
-                if (!thread_wait(bar(PB_ITEMFULL + (seq & 1)), (seq >> 1) & 1, ctl, W + 8)) break;
-                read_item(seq, w);
-                mbar_arrive(bar(PB_ITEMEMPTY + (seq & 1)));
-                if (w.head < 0) break;
-                const int n = max(w.n0, w.n1), mine = t ? w.n1 : w.n0;
-                if (n == 0) continue;
-                const int qb = n_q % NQ;
-                if (!thread_wait(bar(PB_QFULL + qb), (n_q / NQ) & 1, ctl, W + 9)) break;
-                ++n_q;
-                if (mine == 0) mbar_arrive(bar(PB_QEMPTY + qb));
-                const uint64_t dQ = dQ0 + ((qb * 2 * L::kQTile) >> 4);
-                int s_next = 0, o_next = 0;
-                long long t0 = 0;
-                while (o_next < mine) {
-                    bool went = false;
-                    if (s_next < mine && s_next < o_next + 2) {
-                        const uint32_t x = g + s_next, st = x % NS, s = steps + s_next, b = s & 1;
-                        // (the product that read the P which this S overwrites is done)
-                        if ((s < 2 || mbar_test(bar(PB_PVDONE + t * 2 + b), ((s >> 1) - 1) & 1)) && mbar_test(bar(PB_KFULL + st), (x / NS) & 1)) {
+                        for (int t = 0; t < 2; ++t) {
+                            if (next[t] >= min(need[t], there)) continue;
+                            const uint32_t st = (g + next[t]) % NS, s = steps[t] + next[t], b = s & 1;
+                            // its buffer is free: S of two steps before is in registers, or over it P has been read
+                            if (s >= 2 && !mbar_test(bar((L::kOverlay ? PB_PVDONE : PB_SFREE) + t * 2 + b), ((s >> 1) - 1) & 1)) continue;
                             tc_fence_after();
 #pragma unroll
                             for (int k = 0; k < HD / 16; ++k)
-                                umma_ss(tmem + (t * 2 + b) * kKeys, dQ + (((k >> 2) * L::kQChunk + (k & 3) * 32) >> 4),
-                                        dK0 + ((st * L::kTile + (k >> 2) * L::kKChunk + (k & 3) * 32) >> 4), idesc1, k > 0 ? 1u : 0u);
-                            umma_commit(bar(PB_KEMPTY + st));
+                                umma_ss(tmem + (t * 2 + b) * kKeys, dQ0 + (((qb * 2 + t) * L::kQTile + (k >> 2) * L::kQChunk + (k & 3) * 32) >> 4),
+                                        dK0 + ((st * L::kTile + (k >> 2) * L::kKChunk + (k & 3) * 32) >> 4), idesc, k > 0 ? 1u : 0u);
                             umma_commit(bar(PB_SFULL + t * 2 + b));
-                            if (++s_next == mine) umma_commit(bar(PB_QEMPTY + qb));
+                            ++next[t];
                             went = true;
                         }
-                    }
-                    {
-                        const uint32_t x = g + o_next, st = x % NS, s = steps + o_next, b = s & 1;
-                        if (o_next < s_next && mbar_test(bar(PB_PFULL + t * 2 + b), (s >> 1) & 1) && mbar_test(bar(PB_VFULL + st), (x / NS) & 1) &&
-                            (o_next > 0 || outs == 0 || mbar_test(bar(PB_OFREE + t), (outs - 1) & 1))) {
-                            tc_fence_after();
-#pragma unroll
-                            for (int k = 0; k < kKeys / 16; ++k)
-                                umma_ts(tO, tmem + (t * 2 + b) * kKeys + k * 8, dV0 + st * (L::kTile >> 4) + k * 128, idesc2, (o_next > 0 || k > 0) ? 1u : 0u);
-                            umma_commit(bar(PB_VEMPTY + st));
-                            umma_commit(bar(PB_PVDONE + t * 2 + b));
-                            if (++o_next == mine) umma_commit(bar(PB_OFULL + t));
-                            went = true;
+                        while (back < there && next[0] >= min(need[0], back + 1) && next[1] >= min(need[1], back + 1)) {
+                            umma_commit(bar(PB_KEMPTY + (g + back) % NS));
+                            if (++back == n) umma_commit(bar(PB_QEMPTY + qb));
+                        }
+                        if (went) t0 = 0;
+                        else if (t0 == 0) t0 = clock64();
+                        else if (*abort_flag) { ok = false; break; }
+                        else if (clock64() - t0 > args.wait.limit_cycles) {
+                            *abort_flag = 1;
+                            atomicCAS(args.wait.status, 0, W + 10);
+                            atomicExch(args.wait.abort_seq, args.wait.seq);
+                            ok = false;
+                            break;
                         }
                     }
-                    if (went) t0 = 0;
-                    else if (t0 == 0) t0 = clock64();
-                    else if (*abort_flag) { ok = false; break; }
-                    else if (clock64() - t0 > args.wait.limit_cycles) {
-                        *abort_flag = 1;
-                        atomicCAS(args.wait.status, 0, W + 10);
-                        atomicExch(args.wait.abort_seq, args.wait.seq);
-                        ok = false;
-                        break;
-                    }
+                    g += n;
+                    steps[0] += w.n0;
+                    steps[1] += w.n1;
                 }
-                // the other tile of rows goes on alone: every phase is still seen, and every stage given back
-                for (int j = mine; ok && j < n; ++j) {
-                    const uint32_t st = (g + j) % NS, lap = ((g + j) / NS) & 1;
-                    ok = thread_wait(bar(PB_KFULL + st), lap, ctl, W + 11) && thread_wait(bar(PB_VFULL + st), lap, ctl, W + 12);
-                    mbar_arrive(bar(PB_KEMPTY + st));
-                    mbar_arrive(bar(PB_VEMPTY + st));
+            }
+        } else {
+            // -------------------------------------------------------------- O += P V of one tile of rows
+            const int t = warp - kIssue - 1;
+            constexpr uint32_t idesc = umma_idesc(kRows, HD, false, true);
+            const uint64_t dV0 = desc_mnmajor(sV, L::kKChunk);
+            const uint32_t tP = tmem + L::kColP + t * 2 * L::kPStride, tO = tmem + L::kColO + t * L::kOStride;
+            PromptItem w;
+            uint32_t g = 0, steps = 0, seen = 0;      // (seen: parities of the stages' raw barriers, which only tiles with the end of a sequence use)
+            int outs = 0;
+            bool ok = true;
+            for (int seq = 0; ok && next_item(seq, w); ++seq) {
+                const int n = max(w.n0, w.n1), mine = t ? w.n1 : w.n0;
+                for (int j = 0; j < n; ++j) {
+                    const uint32_t st = (g + j) % NS, lap = ((g + j) / NS) & 1, s = steps + j, b = s & 1;
+                    if (t == 0 && (j + 1) * kKeys > w.lk) {
+                        if (!warp_wait(bar(PB_VRAW + st), seen >> st & 1, ctl, W + 7)) { ok = false; break; }
+                        seen ^= 1u << st;
+                        for (int i = (w.lk - j * kKeys) * 8 + lane; i < kKeys * 8; i += 32)
+#pragma unroll
+                            for (int c = 0; c < L::kChunks; ++c) st_shared_v4(sV + st * L::kTile + c * L::kKChunk + i * 16, 0, 0, 0, 0);
+                        fence_async_smem();
+                        warp_arrive(bar(PB_VFULL + st));
+                    }
+                    if (!warp_wait(bar(PB_VFULL + st), lap, ctl, W + 11)) { ok = false; break; }
+                    if (j >= mine) {       // the other tile of rows goes on alone: every phase is still seen, and every stage given back
+                        if (lane == 0) mbar_arrive(bar(PB_VEMPTY + st));
+                        continue;
+                    }
+                    if (j == 0 && outs > 0 && !warp_wait(bar(PB_OFREE + t), (outs - 1) & 1, ctl, W + 12)) { ok = false; break; }
+                    if (!warp_wait(bar(PB_PFULL + t * 2 + b), (s >> 1) & 1, ctl, W + 13)) { ok = false; break; }
+                    tc_fence_after();
+                    if (lane == 0) {
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            umma_ts(tO, tP + b * L::kPStride + k * 8, dV0 + st * (L::kTile >> 4) + k * 128, idesc, (j > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(bar(PB_PVDONE + t * 2 + b));
+                        umma_commit(bar(PB_VEMPTY + st));
+                        if (j + 1 == mine) umma_commit(bar(PB_OFULL + t));
+                    }
+                    __syncwarp();
                 }
                 g += n;
                 steps += mine;
@@ -413,7 +431,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         constexpr int NO = HD / 2;                   // columns of O that each of the two warpgroups of a tile writes out
         const int t = warp >> 3, par = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t tS = lanes + (t * 2 + par) * kKeys, tO = lanes + L::kColO + t * L::kOStride;
+        const uint32_t tS = lanes + (t * 2 + par) * kKeys, tP = lanes + L::kColP + (t * 2 + par) * L::kPStride, tO = lanes + L::kColO + t * L::kOStride;
         const uint32_t msg_out = bar(PB_MSG + 8 * t + 2 * quarter + par), msg_in = bar(PB_MSG + 8 * t + 2 * quarter + (par ^ 1));
         volatile float *maxima = reinterpret_cast<volatile float *>(gbase + L::kOffMsg) + t * 2 * kRows + row;
         volatile float2 *ends = reinterpret_cast<volatile float2 *>(gbase + L::kOffEnd) + t * 2 * kRows + row;
@@ -427,45 +445,108 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             const int mine = t ? w.n1 : w.n0, r = t * kRows + row;
             const int see = args.causal ? max(0, min(w.lk, w.see + r)) : w.lk;      // keys that this row sees
             const int all = __shfl_sync(0xffffffffu, see, 0);                       // ... and every row of this warp
-            float m = -INFINITY, l = 0.f;                                           // maximum in use, sum of this warpgroup's weights in its scale
+            float m = -INFINITY, l = 0.f;      // the reference that this warpgroup's last step was taken with, and its weights' sum
             for (int j = (steps & 1) ^ par; j < mine; j += 2) {
                 const uint32_t step = steps + j;
                 if (!warp_wait(bar(PB_SFULL + t * 2 + par), (step >> 1) & 1, ctl, W + 15)) { ok = false; break; }
                 tc_fence_after();
-                float s[kKeys];
-                tmem_ld32x2_sync(tS, tS + 32, reinterpret_cast<uint32_t *>(s), reinterpret_cast<uint32_t *>(s) + 32);
-                if (args.negate)
-#pragma unroll
-                    for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
-                if ((j + 1) * kKeys > all) {
-                    const int left = see - j * kKeys;
-#pragma unroll
-                    for (int i = 0; i < kKeys; ++i) s[i] = i < left ? s[i] : -INFINITY;
+                // The product that read what P overwrites is done (over S that is so, or S could not have been computed).  Before the message:
+                // whoever has that knows which phase of this barrier comes next.
+                if (!L::kOverlay && step > 1) {
+                    if (!warp_wait(bar(PB_PVDONE + t * 2 + par), ((step >> 1) - 1) & 1, ctl, W + 14)) { ok = false; break; }
+                    tc_fence_after();
                 }
-                float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int i = 4; i < kKeys; i += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) top[k] = i + 4 < kKeys ? max3(top[k], s[i + k], s[i + 4 + k]) : fmaxf(top[k], s[i + k]);
-                const float x = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-                // the maximum that the step before was taken with (of another item: none)
-                float was = -INFINITY;
-                if (step > 0) {
-                    if (!warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16)) { ok = false; break; }
-                    if (j > 0) was = maxima[(par ^ 1) * kRows];
+                // what the step before was taken with; every message is waited for before the next one is sent
+                bool heard = step == 0;
+                float ref = m;
+                auto hear = [&]() -> bool {
+                    heard = true;
+                    return warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16);
+                };
+                auto send = [&] {
+                    maxima[par * kRows] = ref;
+                    warp_arrive(msg_out);
+                };
+                if (j == 1) {
+                    if (!hear()) { ok = false; break; }
+                    ref = maxima[(par ^ 1) * kRows];
                 }
-                // (the first finite maximum of a row is always taken: -inf is exceeded by more than anything)
-                const bool raise = (x - was) * c > kLazy;
-                const bool any = __any_sync(0xffffffffu, raise);
-                const float now = any ? fmaxf(was, x) : was;
-                maxima[par * kRows] = now;
-                warp_arrive(msg_out);
-                l = m == now ? l : l * (m == -INFINITY ? 0.f : ex2((m - now) * c));
-                m = now;
-                if (any && j > 0) {
+                bool with_max = j == 0;
+                float before = ref, sum;
+                uint32_t p[32];
+                while (true) {
+                    float s[kKeys];
+                    tmem_ld32x2_sync(tS, tS + 32, reinterpret_cast<uint32_t *>(s), reinterpret_cast<uint32_t *>(s) + 32);
+                    if (args.negate)
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
+                    if ((j + 1) * kKeys > all) {
+                        const int left = see - j * kKeys;
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) s[i] = i < left ? s[i] : -INFINITY;
+                    }
+                    if (with_max) {
+                        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                        for (int i = 4; i < kKeys; i += 8)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) top[k] = i + 4 < kKeys ? max3(top[k], s[i + k], s[i + 4 + k]) : fmaxf(top[k], s[i + k]);
+                        before = ref;
+                        ref = fmaxf(ref, fmaxf(max3(top[0], top[1], top[2]), top[3]));
+                        if (!heard && !hear()) { ok = false; break; }
+                        send();          // (no weight of this pass is above 1: it stays)
+                    }
+                    const float mc = ref == -INFINITY ? 0.f : -ref * c;
+                    const f32x2 c2 = f2_pack(c, c), mc2 = f2_pack(mc, mc);
+                    f32x2 sum0 = 0, sum1 = 0;
+#pragma unroll
+                    for (int i = 0; i < kKeys + kLag; i += 8) {
+                        if (i < kKeys) {
+#pragma unroll
+                            for (int k = 0; k < 8; k += 2) {
+                                f2_unpack(f2_fma(f2_pack(s[i + k], s[i + k + 1]), c2, mc2), s[i + k], s[i + k + 1]);
+                                s[i + k] = ex2(s[i + k]);
+                                s[i + k + 1] = ex2(s[i + k + 1]);
+                            }
+                        }
+                        if (i >= kLag) {
+                            const int y = i - kLag;
+#pragma unroll
+                            for (int k = 0; k < 8; k += 4) {
+                                sum0 = f2_add(sum0, f2_pack(s[y + k], s[y + k + 1]));
+                                sum1 = f2_add(sum1, f2_pack(s[y + k + 2], s[y + k + 3]));
+                                p[(y + k) / 2] = pack_bf16(s[y + k], s[y + k + 1]);
+                                p[(y + k) / 2 + 1] = pack_bf16(s[y + k + 2], s[y + k + 3]);
+                            }
+                        }
+                    }
+                    float a0, a1;
+                    f2_unpack(f2_add(sum0, sum1), a0, a1);
+                    sum = a0 + a1;
+                    if (with_max) break;
+                    bool stale = false;
+                    if (!heard) {
+                        if (!hear()) { ok = false; break; }
+                        const float now = maxima[(par ^ 1) * kRows];
+                        stale = now != ref;
+                        ref = now;
+                    }
+                    if (__any_sync(0xffffffffu, stale)) continue;       // the other warpgroup took a new reference: once more with that
+                    with_max = __any_sync(0xffffffffu, sum > kLazy || (ref == -INFINITY && sum > 0.f));
+                    if (!with_max) {
+                        send();
+                        break;
+                    }
+                }
+                if (!ok) break;
+                if (!L::kOverlay) {
+                    tc_fence_before();
+                    warp_arrive(bar(PB_SFREE + t * 2 + par));
+                }
+                if (with_max && j > 0) {
                     if (!warp_wait(bar(PB_PVDONE + t * 2 + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17)) { ok = false; break; }
                     tc_fence_after();
-                    const float keep = was == now ? 1.f : was == -INFINITY ? 0.f : ex2((was - now) * c);
+                    const float keep = before == ref ? 1.f : before == -INFINITY ? 0.f : ex2((before - ref) * c);
 #pragma unroll
                     for (int d = 0; d < HD; d += 16) {
                         uint32_t o[16];
@@ -475,42 +556,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         tmem_st16(tO + d, o);
                     }
                 }
-                const float mc = m == -INFINITY ? 0.f : -m * c;
-                const f32x2 c2 = f2_pack(c, c), mc2 = f2_pack(mc, mc);
-                f32x2 sum0 = 0, sum1 = 0;
-                uint32_t p[16];
-#pragma unroll
-                for (int i = 0; i < kKeys + kLag; i += 8) {
-                    if (i < kKeys) {
-#pragma unroll
-                        for (int k = 0; k < 8; k += 2) {
-                            const f32x2 e = f2_fma(f2_pack(s[i + k], s[i + k + 1]), c2, mc2);
-                            if (k >= 8 - 2 * kByPolynomial) f2_unpack(f2_exp2(e), s[i + k], s[i + k + 1]);
-                            else {
-                                f2_unpack(e, s[i + k], s[i + k + 1]);
-                                s[i + k] = ex2(s[i + k]);
-                                s[i + k + 1] = ex2(s[i + k + 1]);
-                            }
-                        }
-                    }
-                    if (i >= kLag) {
-                        const int y = i - kLag;
-#pragma unroll
-                        for (int k = 0; k < 8; k += 4) {
-                            sum0 = f2_add(sum0, f2_pack(s[y + k], s[y + k + 1]));
-                            sum1 = f2_add(sum1, f2_pack(s[y + k + 2], s[y + k + 3]));
-                            p[((y + k) & 31) / 2] = pack_bf16(s[y + k], s[y + k + 1]);
-                            p[((y + k) & 31) / 2 + 1] = pack_bf16(s[y + k + 2], s[y + k + 3]);
-                        }
-                        if ((y & 31) == 24) tmem_st16(tS + y / 32 * 16, p);
-                    }
-                }
-                float a0, a1;
-                f2_unpack(f2_add(sum0, sum1), a0, a1);
-                l += a0 + a1;
+                tmem_st32(tP, p);
                 tmem_st_wait();
                 tc_fence_before();
                 warp_arrive(bar(PB_PFULL + t * 2 + par));
+                l = fmaf(l, m == ref ? 1.f : m == -INFINITY ? 0.f : ex2((m - ref) * c), sum);
+                m = ref;
             }
             steps += mine;
             if (!ok) break;
