@@ -32,40 +32,40 @@
 namespace fmhf {
 namespace {
 
-constexpr int kRows = 128, kItemRows = 2 * kRows, kKeys = 64;
-constexpr int kSoftmaxWarps = 16, kThreads = (kSoftmaxWarps + 4) * 32;
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 4) * 32;
 constexpr int kKernelPrompt = 6;                  // status codes 601..
 constexpr float kLazy = 65536.f;                  // the sum of a row's weights of a step above which its reference is set anew
 constexpr int kLag = 8;
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 4;
 
 template <int HD>
 struct PromptCfg {
-    static constexpr int kChunks = (HD + 63) / 64, kStages = HD == 64 ? 8 : 4, kQBufs = HD == 64 ? 2 : 1;
-    static constexpr uint32_t kQChunk = kRows * 128, kKChunk = kKeys * 128;     // 64 columns of a tile
-    static constexpr uint32_t kQTile = kChunks * kQChunk, kTile = kChunks * kKChunk;
-    static constexpr uint32_t kOffQ = 0, kOffK = kQBufs * 2 * kQTile, kOffV = kOffK + kStages * kTile;
-    static constexpr uint32_t kOffMsg = kOffV + kStages * kTile, kOffEnd = kOffMsg + 4 * kRows * 4;   // [tile][parity][row]: maxima; maxima and sums (of two items)
-    static constexpr uint32_t kOffBar = kOffEnd + 2 * 4 * kRows * 8, kTotal = kOffBar + 1024 + 1024;
-    // tensor memory: two buffers for S of either tile of rows, O of both, and P: over S, or by itself where there is room
-    static constexpr bool kOverlay = HD != 64;
-    static constexpr uint32_t kColP = kOverlay ? 0 : 256, kPStride = kOverlay ? kKeys : kKeys / 2, kColO = kOverlay ? 256 : 384, kOStride = HD == 64 ? 64 : 128;
+    static constexpr int kChunks = (HD + 63) / 64, kStages = HD == 64 ? 4 : 2;
+    static constexpr uint32_t kChunk = kRows * 128;             // 64 columns of a tile
+    static_assert(kRows == kKeys, "tiles of Q, K and V are of one size");
+    static constexpr uint32_t kTile = kChunks * kChunk;
+    static constexpr uint32_t kOffQ = 0, kOffK = 2 * kTile, kOffV = kOffK + kStages * kTile;
+    static constexpr uint32_t kOffMsg = kOffV + kStages * kTile, kOffEnd = kOffMsg + 2 * kRows * 4;   // [parity][row]: references; those and sums (of two items)
+    static constexpr uint32_t kOffBar = kOffEnd + 2 * 2 * kRows * 8, kTotal = kOffBar + 512 + 1024;
 };
+// Tensor memory: two buffers for S, two for P (two bf16 a column), O.
+constexpr uint32_t kColP = 256, kColO = 384;
 
-// SFULL: S computed into a buffer; SFREE: it is in registers; PFULL: P written, O scaled if need be; PVDONE: the product that read P is done (tile
-// t, buffer b: + 2 t + b); OFULL: the last one of an item; OFREE: O has been read out (+ t); MSG: the maximum that a step was taken with (tile t, quarter q,
-// steps of parity b: + 8 t + 2 q + b); ITEM*: the ring of work items; NEXT: the answer to a request for one.
-enum { PB_QFULL = 0, PB_QEMPTY = 2, PB_SFULL = 4, PB_PFULL = 8, PB_PVDONE = 12, PB_OFULL = 16, PB_OFREE = 18, PB_ITEMFULL = 20, PB_ITEMEMPTY = 22,
-       PB_NEXT = 24, PB_MSG = 25, PB_SFREE = 41, PB_KFULL = 45, PB_KEMPTY = PB_KFULL + kMaxStages, PB_VFULL = PB_KEMPTY + kMaxStages,
+// SFULL: S computed into a buffer; SFREE: it is in registers; PFULL: P written, O scaled if need be; PVDONE: the product that read P is done (+
+// buffer); OFULL: the last one of an item; OFREE: O has been read out; MSG: the reference that a step was taken with (quarter q, steps of parity
+// b: + 2 q + b); ITEM*: the ring of work items; NEXT: the answer to a request for one.
+enum { PB_QFULL = 0, PB_QEMPTY = 2, PB_SFULL = 4, PB_SFREE = 6, PB_PFULL = 8, PB_PVDONE = 10, PB_OFULL = 12, PB_OFREE = 13, PB_ITEMFULL = 14,
+       PB_ITEMEMPTY = 16, PB_NEXT = 18, PB_MSG = 19, PB_KFULL = 27, PB_KEMPTY = PB_KFULL + kMaxStages, PB_VFULL = PB_KEMPTY + kMaxStages,
        PB_VEMPTY = PB_VFULL + kMaxStages, PB_VRAW = PB_VEMPTY + kMaxStages, PB_COUNT = PB_VRAW + kMaxStages };
 constexpr uint32_t kOffNext = (PB_COUNT * 8 + 15) / 16 * 16, kOffItems = kOffNext + 16, kOffCtl = kOffItems + 2 * 48;
-static_assert(kOffCtl + 8 <= 1024, "control area");
+static_assert(kOffCtl + 8 <= 512, "control area");
 
 struct PromptItem {
     int q0, lq;          // first row of the item in the packed rows; rows of the sequence from there on
     int k0, lk;          // first key and keys of the sequence
     int see;             // keys that the item's first row sees, before clamping: row r sees min(lk, see + r) (causal) or lk
-    int n0, n1;          // tiles of keys for the two tiles of rows
+    int n;               // tiles of keys
     int head;            // -1: no more items
 };
 
@@ -81,14 +81,14 @@ struct PromptArgs {
 };
 
 // Item `index`: the last rows of each sequence, which see the most keys when the call is causal, come first.  Sequence b owns the slots
-// from cu[b] / 256 + b on, at least as many as it has items.
+// from cu[b] / 128 + b on, at least as many as it has items.
 __device__ __forceinline__ bool prompt_item(const PromptArgs &a, int index, PromptItem &w) {
-    const int slots = a.tokens_q / kItemRows + a.B, slot = slots - 1 - index / a.n_q;
+    const int slots = a.tokens_q / kRows + a.B, slot = slots - 1 - index / a.n_q;
     w.head = index % a.n_q;
     int lo = 0, hi = a.B - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(a.cu_q + mid) / kItemRows + mid <= slot) lo = mid;
+        if (__ldg(a.cu_q + mid) / kRows + mid <= slot) lo = mid;
         else hi = mid - 1;
     }
     const int q0 = __ldg(a.cu_q + lo), q1 = __ldg(a.cu_q + lo + 1), k0 = __ldg(a.cu_k + lo), k1 = __ldg(a.cu_k + lo + 1);
@@ -96,21 +96,15 @@ __device__ __forceinline__ bool prompt_item(const PromptArgs &a, int index, Prom
         note_index(a.wait.status, kPromptRows);
         return false;
     }
-    const int r0 = (slot - (q0 / kItemRows + lo)) * kItemRows, lq = q1 - q0, lk = k1 - k0;
+    const int r0 = (slot - (q0 / kRows + lo)) * kRows, lq = q1 - q0, lk = k1 - k0;
     if (r0 < 0 || r0 >= lq) return false;
     w.q0 = q0 + r0;
     w.lq = lq - r0;
     w.k0 = k0;
     w.lk = lk;
     w.see = a.causal ? r0 + 1 + lk - lq : lk;
-    auto tiles = [&](int first, int rows) {      // tiles of keys that rows first .. first + rows - 1 need
-        rows = min(rows, w.lq - first);
-        if (rows <= 0) return 0;
-        const int most = a.causal ? min(lk, max(0, w.see + first + rows - 1)) : lk;
-        return (most + kKeys - 1) / kKeys;
-    };
-    w.n0 = tiles(0, kRows);
-    w.n1 = tiles(kRows, kRows);
+    const int most = a.causal ? min(lk, max(0, w.see + min(kRows, w.lq) - 1)) : lk;      // keys that the last row sees
+    w.n = (most + kKeys - 1) / kKeys;
     return true;
 }
 
@@ -129,26 +123,6 @@ __device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-// 2^x of both halves on the FMA pipe: x = n + f, n whole, |f| <= 1/2 (adding 1.5 * 2^23 rounds x to n and leaves it in the low bits), and a cubic in f of
-// relative error 7.5e-5 at most, a fiftieth of the rounding of P to bf16 (fitted here: least squares in the relative error, reweighted
-// until its extremes were level).  Below 2^-126 the result is 2^-126 or so, not 0: nothing beside a largest P of 1, but a row that
-// sees nothing has to be known by its maximum.  What is not a number becomes so large that no finite result is left.
-__device__ __forceinline__ f32x2 f2_exp2(f32x2 x) {
-    float a, b, u, v;
-    f2_unpack(x, a, b);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
-    x = f2_pack(a, b);
-    const f32x2 magic = f2_pack(12582912.f, 12582912.f), back = f2_pack(-12582912.f, -12582912.f), minus = f2_pack(-1.f, -1.f);
-    const f32x2 r = f2_add(x, magic), f = f2_fma(f2_add(r, back), minus, x);
-    f32x2 y = f2_fma(f2_pack(0.0551716685f, 0.0551716685f), f, f2_pack(0.242611125f, 0.242611125f));
-    y = f2_fma(y, f, f2_pack(0.693260968f, 0.693260968f));
-    y = f2_fma(y, f, f2_pack(0.999928057f, 0.999928057f));
-    f2_unpack(r, a, b);
-    f2_unpack(y, u, v);
-    return f2_pack(__int_as_float(__float_as_int(u) + (__float_as_int(a) << 23)), __int_as_float(__float_as_int(v) + (__float_as_int(b) << 23)));
-}
-
 // Bounded waits, in line: a call would spill what a softmax thread holds.  Of one thread; and of a whole warp, with the same answer for all lanes
 // (those of a warp that gives up leave its loop together).
 __device__ __forceinline__ bool thread_wait(uint32_t bar, uint32_t parity, const WaitCtl &ctl, int code) {
@@ -180,12 +154,24 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const W
     }
 }
 
+// A thread's row of S, all of it behind one wait.
+__device__ __forceinline__ void tmem_row(uint32_t ta, uint32_t *a) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%128];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%129];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(a[16]), "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]), "=r"(a[24]), "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]), "=r"(a[32]), "=r"(a[33]), "=r"(a[34]), "=r"(a[35]), "=r"(a[36]), "=r"(a[37]), "=r"(a[38]), "=r"(a[39]), "=r"(a[40]), "=r"(a[41]), "=r"(a[42]), "=r"(a[43]), "=r"(a[44]), "=r"(a[45]), "=r"(a[46]), "=r"(a[47]), "=r"(a[48]), "=r"(a[49]), "=r"(a[50]), "=r"(a[51]), "=r"(a[52]), "=r"(a[53]), "=r"(a[54]), "=r"(a[55]), "=r"(a[56]), "=r"(a[57]), "=r"(a[58]), "=r"(a[59]), "=r"(a[60]), "=r"(a[61]), "=r"(a[62]), "=r"(a[63]),
+          "=r"(a[64]), "=r"(a[65]), "=r"(a[66]), "=r"(a[67]), "=r"(a[68]), "=r"(a[69]), "=r"(a[70]), "=r"(a[71]), "=r"(a[72]), "=r"(a[73]), "=r"(a[74]), "=r"(a[75]), "=r"(a[76]), "=r"(a[77]), "=r"(a[78]), "=r"(a[79]), "=r"(a[80]), "=r"(a[81]), "=r"(a[82]), "=r"(a[83]), "=r"(a[84]), "=r"(a[85]), "=r"(a[86]), "=r"(a[87]), "=r"(a[88]), "=r"(a[89]), "=r"(a[90]), "=r"(a[91]), "=r"(a[92]), "=r"(a[93]), "=r"(a[94]), "=r"(a[95]), "=r"(a[96]), "=r"(a[97]), "=r"(a[98]), "=r"(a[99]), "=r"(a[100]), "=r"(a[101]), "=r"(a[102]), "=r"(a[103]), "=r"(a[104]), "=r"(a[105]), "=r"(a[106]), "=r"(a[107]), "=r"(a[108]), "=r"(a[109]), "=r"(a[110]), "=r"(a[111]), "=r"(a[112]), "=r"(a[113]), "=r"(a[114]), "=r"(a[115]), "=r"(a[116]), "=r"(a[117]), "=r"(a[118]), "=r"(a[119]), "=r"(a[120]), "=r"(a[121]), "=r"(a[122]), "=r"(a[123]), "=r"(a[124]), "=r"(a[125]), "=r"(a[126]), "=r"(a[127])
+        : "r"(ta), "r"(ta + 64)
+        : "memory");
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const PromptArgs args) {
     using L = PromptCfg<HD>;
-    constexpr int NS = L::kStages, NQ = L::kQBufs;
+    constexpr int NS = L::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -204,24 +190,22 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(PB_QFULL + i), 1);
             mbar_init(bar(PB_QEMPTY + i), 1);
-            mbar_init(bar(PB_OFULL + i), 1);
-            mbar_init(bar(PB_OFREE + i), 8);
-            mbar_init(bar(PB_ITEMFULL + i), 1);
-            mbar_init(bar(PB_ITEMEMPTY + i), kSoftmaxWarps + 3);      // every warp but the one that fills it
-        }
-        for (int i = 0; i < 4; ++i) {
             mbar_init(bar(PB_SFULL + i), 1);
-            mbar_init(bar(PB_PFULL + i), 4);
             mbar_init(bar(PB_SFREE + i), 4);
+            mbar_init(bar(PB_PFULL + i), 4);
             mbar_init(bar(PB_PVDONE + i), 1);
+            mbar_init(bar(PB_ITEMFULL + i), 1);
+            mbar_init(bar(PB_ITEMEMPTY + i), kSoftmaxWarps + 2);      // every warp but the one that fills it
         }
-        for (int i = 0; i < 16; ++i) mbar_init(bar(PB_MSG + i), 1);
+        mbar_init(bar(PB_OFULL), 1);
+        mbar_init(bar(PB_OFREE), 8);
+        for (int i = 0; i < 8; ++i) mbar_init(bar(PB_MSG + i), 1);
         mbar_init(bar(PB_NEXT), 1);
         for (int i = 0; i < NS; ++i) {
             mbar_init(bar(PB_KFULL + i), 1);
             mbar_init(bar(PB_KEMPTY + i), 1);
             mbar_init(bar(PB_VFULL + i), 1);
-            mbar_init(bar(PB_VEMPTY + i), 2);
+            mbar_init(bar(PB_VEMPTY + i), 1);
             mbar_init(bar(PB_VRAW + i), 1);
         }
         fence_mbar_init();
@@ -235,7 +219,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     // Work item `seq` of this block, after a wait for it.
     auto read_item = [&](int seq, PromptItem &w) {
         volatile int *p = items + (seq & 1) * 12;
-        w.q0 = p[0]; w.lq = p[1]; w.k0 = p[2]; w.lk = p[3]; w.see = p[4]; w.n0 = p[5]; w.n1 = p[6]; w.head = p[7];
+        w.q0 = p[0]; w.lq = p[1]; w.k0 = p[2]; w.lk = p[3]; w.see = p[4]; w.n = p[5]; w.head = p[6];
     };
     auto next_item = [&](int seq, PromptItem &w) -> bool {       // for a whole warp; false: no more, or given up
         if (!warp_wait(bar(PB_ITEMFULL + (seq & 1)), (seq >> 1) & 1, ctl, W + 1)) return false;
@@ -247,8 +231,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     if (*abort_flag) {
         // nothing: fall through to the teardown
     } else if (warp >= kSoftmaxWarps) {
-        // A softmax thread holds a row of S: 512 x 104 + 128 x 56 registers of the 640 x 96 that the launch has.
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        // A softmax thread holds a row of S: 256 x 208 + 128 x 88 registers, the 384 x 168 that the launch has.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == kLoad) {
             // -------------------------------------------------------------- work items and TMA
             if (lane == 0) {
@@ -274,20 +258,19 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         const int s = seq & 1;
                         if (seq >= 2 && !thread_wait(bar(PB_ITEMEMPTY + s), ((seq >> 1) - 1) & 1, ctl, W + 2)) break;
                         volatile int *p = items + s * 12;
-                        p[0] = w.q0; p[1] = w.lq; p[2] = w.k0; p[3] = w.lk; p[4] = w.see; p[5] = w.n0; p[6] = w.n1; p[7] = w.head;
+                        p[0] = w.q0; p[1] = w.lq; p[2] = w.k0; p[3] = w.lk; p[4] = w.see; p[5] = w.n; p[6] = w.head;
                         mbar_arrive(bar(PB_ITEMFULL + s));
                         ++seq;
                     }
                     if (index < 0) break;
-                    const int n = w.head < 0 ? 0 : max(w.n0, w.n1);
+                    const int n = w.head < 0 ? 0 : w.n;
                     if (n > 0) {
-                        const int qb = n_q % NQ;
-                        if (n_q >= NQ && !thread_wait(bar(PB_QEMPTY + qb), (n_q / NQ - 1) & 1, ctl, W + 3)) break;
+                        const int qb = n_q & 1;
+                        if (n_q >= 2 && !thread_wait(bar(PB_QEMPTY + qb), ((n_q >> 1) - 1) & 1, ctl, W + 3)) break;
                         ++n_q;
-                        mbar_arrive_expect_tx(bar(PB_QFULL + qb), ((w.n0 > 0) + (w.n1 > 0)) * L::kQTile);
-                        for (int t = 0; t < 2; ++t)
-                            for (int c = 0; c < ((t ? w.n1 : w.n0) > 0 ? L::kChunks : 0); ++c)
-                                tma_load_3d(sQ + (qb * 2 + t) * L::kQTile + c * L::kQChunk, &tmQ, bar(PB_QFULL + qb), c * 64, w.head, w.q0 + t * kRows);
+                        mbar_arrive_expect_tx(bar(PB_QFULL + qb), L::kTile);
+                        for (int c = 0; c < L::kChunks; ++c)
+                            tma_load_3d(sQ + qb * L::kTile + c * L::kChunk, &tmQ, bar(PB_QFULL + qb), c * 64, w.head, w.q0);
                     }
                     const int kh = w.head / args.group;
                     for (int j = 0; j < n; ++j, ++g) {
@@ -295,11 +278,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         if (!thread_wait(bar(PB_KEMPTY + st), lap ^ 1, ctl, W + 4)) { ok = false; break; }
                         mbar_arrive_expect_tx(bar(PB_KFULL + st), L::kTile);
                         for (int c = 0; c < L::kChunks; ++c)
-                            tma_load_3d(sK + st * L::kTile + c * L::kKChunk, &tmK, bar(PB_KFULL + st), c * 64, kh, w.k0 + j * kKeys);
+                            tma_load_3d(sK + st * L::kTile + c * L::kChunk, &tmK, bar(PB_KFULL + st), c * 64, kh, w.k0 + j * kKeys);
                         if (!thread_wait(bar(PB_VEMPTY + st), lap ^ 1, ctl, W + 5)) { ok = false; break; }
                         const uint32_t full = bar(((j + 1) * kKeys > w.lk ? PB_VRAW : PB_VFULL) + st);
                         mbar_arrive_expect_tx(full, L::kTile);
-                        for (int c = 0; c < L::kChunks; ++c) tma_load_3d(sV + st * L::kTile + c * L::kKChunk, &tmV, full, c * 64, kh, w.k0 + j * kKeys);
+                        for (int c = 0; c < L::kChunks; ++c) tma_load_3d(sV + st * L::kTile + c * L::kChunk, &tmV, full, c * 64, kh, w.k0 + j * kKeys);
                     }
                     if (!ok || !thread_wait(bar(PB_NEXT), asked++ & 1, ctl, W + 6)) break;
                     uint32_t got, next;
@@ -315,12 +298,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 }
             }
         } else if (warp == kIssue) {
-            // -------------------------------------------------------------- S of both tiles, whichever can go on
+            // -------------------------------------------------------------- S = Q K^T
             if (lane == 0) {
                 constexpr uint32_t idesc = umma_idesc(kRows, kKeys, false, false);
                 const uint64_t dQ0 = desc_kmajor(sQ), dK0 = desc_kmajor(sK);
                 PromptItem w;
-                uint32_t g = 0, steps[2] = {0, 0};      // tiles of keys so far, of all items; those that the tiles of rows needed
+                uint32_t s = 0;           // steps so far, of all items
                 int n_q = 0;
                 bool ok = true;
                 for (int seq = 0; ok; ++seq) {
@@ -328,132 +311,93 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     read_item(seq, w);
                     mbar_arrive(bar(PB_ITEMEMPTY + (seq & 1)));
                     if (w.head < 0) break;
-                    const int n = max(w.n0, w.n1), need[2] = {w.n0, w.n1};
-                    if (n == 0) continue;
-                    const int qb = n_q % NQ;
-                    if (!thread_wait(bar(PB_QFULL + qb), (n_q / NQ) & 1, ctl, W + 9)) break;
+                    if (w.n == 0) continue;
+                    const int qb = n_q & 1;
+                    if (!thread_wait(bar(PB_QFULL + qb), (n_q >> 1) & 1, ctl, W + 9)) break;
                     ++n_q;
-                    int next[2] = {0, 0}, there = 0, back = 0;      // S issued; tiles of keys that have come, that were given back
-                    long long t0 = 0;
-                    while (back < n) {
-                        bool went = false;
-                        if (there < n && there <= max(next[0], next[1])) {
-                            const uint32_t x = g + there;
-                            if (mbar_test(bar(PB_KFULL + x % NS), (x / NS) & 1)) {
-                                ++there;
-                                went = true;
-                            }
-                        }
+                    for (int j = 0; j < w.n; ++j, ++s) {
+                        const uint32_t st = s % NS, b = s & 1;
+                        if (!thread_wait(bar(PB_KFULL + st), (s / NS) & 1, ctl, W + 10)) { ok = false; break; }
+                        // its buffer is free: S of two steps before is in registers
+                        if (s >= 2 && !thread_wait(bar(PB_SFREE + b), ((s >> 1) - 1) & 1, ctl, W + 11)) { ok = false; break; }
+                        tc_fence_after();
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            if (next[t] >= min(need[t], there)) continue;
-                            const uint32_t st = (g + next[t]) % NS, s = steps[t] + next[t], b = s & 1;
-                            // its buffer is free: S of two steps before is in registers, or over it P has been read
-                            if (s >= 2 && !mbar_test(bar((L::kOverlay ? PB_PVDONE : PB_SFREE) + t * 2 + b), ((s >> 1) - 1) & 1)) continue;
-                            tc_fence_after();
-#pragma unroll
-                            for (int k = 0; k < HD / 16; ++k)
-                                umma_ss(tmem + (t * 2 + b) * kKeys, dQ0 + (((qb * 2 + t) * L::kQTile + (k >> 2) * L::kQChunk + (k & 3) * 32) >> 4),
-                                        dK0 + ((st * L::kTile + (k >> 2) * L::kKChunk + (k & 3) * 32) >> 4), idesc, k > 0 ? 1u : 0u);
-                            umma_commit(bar(PB_SFULL + t * 2 + b));
-                            ++next[t];
-                            went = true;
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint32_t off = (k >> 2) * L::kChunk + (k & 3) * 32;
+                            umma_ss(tmem + b * kKeys, dQ0 + ((qb * L::kTile + off) >> 4), dK0 + ((st * L::kTile + off) >> 4), idesc, k > 0 ? 1u : 0u);
                         }
-                        while (back < there && next[0] >= min(need[0], back + 1) && next[1] >= min(need[1], back + 1)) {
-                            umma_commit(bar(PB_KEMPTY + (g + back) % NS));
-                            if (++back == n) umma_commit(bar(PB_QEMPTY + qb));
-                        }
-                        if (went) t0 = 0;
-                        else if (t0 == 0) t0 = clock64();
-                        else if (*abort_flag) { ok = false; break; }
-                        else if (clock64() - t0 > args.wait.limit_cycles) {
-                            *abort_flag = 1;
-                            atomicCAS(args.wait.status, 0, W + 10);
-                            atomicExch(args.wait.abort_seq, args.wait.seq);
-                            ok = false;
-                            break;
-                        }
+                        umma_commit(bar(PB_SFULL + b));
+                        umma_commit(bar(PB_KEMPTY + st));
+                        if (j + 1 == w.n) umma_commit(bar(PB_QEMPTY + qb));
                     }
-                    g += n;
-                    steps[0] += w.n0;
-                    steps[1] += w.n1;
                 }
             }
-        } else {
-            // -------------------------------------------------------------- O += P V of one tile of rows
-            const int t = warp - kIssue - 1;
+        } else if (warp == kIssue + 1) {
+            // -------------------------------------------------------------- O += P V
             constexpr uint32_t idesc = umma_idesc(kRows, HD, false, true);
-            const uint64_t dV0 = desc_mnmajor(sV, L::kKChunk);
-            const uint32_t tP = tmem + L::kColP + t * 2 * L::kPStride, tO = tmem + L::kColO + t * L::kOStride;
+            const uint64_t dV0 = desc_mnmajor(sV, L::kChunk);
             PromptItem w;
-            uint32_t g = 0, steps = 0, seen = 0;      // (seen: parities of the stages' raw barriers, which only tiles with the end of a sequence use)
+            uint32_t s = 0, seen = 0;      // steps so far; parities of the stages' raw barriers, which only tiles with the end of a sequence use
             int outs = 0;
             bool ok = true;
             for (int seq = 0; ok && next_item(seq, w); ++seq) {
-                const int n = max(w.n0, w.n1), mine = t ? w.n1 : w.n0;
-                for (int j = 0; j < n; ++j) {
-                    const uint32_t st = (g + j) % NS, lap = ((g + j) / NS) & 1, s = steps + j, b = s & 1;
-                    if (t == 0 && (j + 1) * kKeys > w.lk) {
+                for (int j = 0; j < w.n; ++j, ++s) {
+                    const uint32_t st = s % NS, b = s & 1;
+                    if ((j + 1) * kKeys > w.lk) {
                         if (!warp_wait(bar(PB_VRAW + st), seen >> st & 1, ctl, W + 7)) { ok = false; break; }
                         seen ^= 1u << st;
                         for (int i = (w.lk - j * kKeys) * 8 + lane; i < kKeys * 8; i += 32)
 #pragma unroll
-                            for (int c = 0; c < L::kChunks; ++c) st_shared_v4(sV + st * L::kTile + c * L::kKChunk + i * 16, 0, 0, 0, 0);
+                            for (int c = 0; c < L::kChunks; ++c) st_shared_v4(sV + st * L::kTile + c * L::kChunk + i * 16, 0, 0, 0, 0);
                         fence_async_smem();
                         warp_arrive(bar(PB_VFULL + st));
                     }
-                    if (!warp_wait(bar(PB_VFULL + st), lap, ctl, W + 11)) { ok = false; break; }
-                    if (j >= mine) {       // the other tile of rows goes on alone: every phase is still seen, and every stage given back
-                        if (lane == 0) mbar_arrive(bar(PB_VEMPTY + st));
-                        continue;
-                    }
-                    if (j == 0 && outs > 0 && !warp_wait(bar(PB_OFREE + t), (outs - 1) & 1, ctl, W + 12)) { ok = false; break; }
-                    if (!warp_wait(bar(PB_PFULL + t * 2 + b), (s >> 1) & 1, ctl, W + 13)) { ok = false; break; }
+                    if (!warp_wait(bar(PB_VFULL + st), (s / NS) & 1, ctl, W + 12)) { ok = false; break; }
+                    if (j == 0 && outs > 0 && !warp_wait(bar(PB_OFREE), (outs - 1) & 1, ctl, W + 13)) { ok = false; break; }
+                    if (!warp_wait(bar(PB_PFULL + b), (s >> 1) & 1, ctl, W + 14)) { ok = false; break; }
                     tc_fence_after();
                     if (lane == 0) {
 #pragma unroll
                         for (int k = 0; k < kKeys / 16; ++k)
-                            umma_ts(tO, tP + b * L::kPStride + k * 8, dV0 + st * (L::kTile >> 4) + k * 128, idesc, (j > 0 || k > 0) ? 1u : 0u);
-                        umma_commit(bar(PB_PVDONE + t * 2 + b));
+                            umma_ts(tmem + kColO, tmem + kColP + b * (kKeys / 2) + k * 8, dV0 + st * (L::kTile >> 4) + k * 128, idesc,
+                                    (j > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(bar(PB_PVDONE + b));
                         umma_commit(bar(PB_VEMPTY + st));
-                        if (j + 1 == mine) umma_commit(bar(PB_OFULL + t));
+                        if (j + 1 == w.n) umma_commit(bar(PB_OFULL));
                     }
                     __syncwarp();
                 }
-                g += n;
-                steps += mine;
-                outs += mine > 0;
+                outs += w.n > 0;
             }
         }
     } else {
         // ------------------------------------------------------------------ softmax and output, a thread a row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         constexpr int NO = HD / 2;                   // columns of O that each of the two warpgroups of a tile writes out
-        const int t = warp >> 3, par = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
+        const int par = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t tS = lanes + (t * 2 + par) * kKeys, tP = lanes + L::kColP + (t * 2 + par) * L::kPStride, tO = lanes + L::kColO + t * L::kOStride;
-        const uint32_t msg_out = bar(PB_MSG + 8 * t + 2 * quarter + par), msg_in = bar(PB_MSG + 8 * t + 2 * quarter + (par ^ 1));
-        volatile float *maxima = reinterpret_cast<volatile float *>(gbase + L::kOffMsg) + t * 2 * kRows + row;
-        volatile float2 *ends = reinterpret_cast<volatile float2 *>(gbase + L::kOffEnd) + t * 2 * kRows + row;
-        const int pair_bar = 1 + (t * 4 + quarter);
+        const uint32_t tS = lanes + par * kKeys, tP = lanes + kColP + par * (kKeys / 2), tO = lanes + kColO;
+        const uint32_t msg_out = bar(PB_MSG + 2 * quarter + par), msg_in = bar(PB_MSG + 2 * quarter + (par ^ 1));
+        volatile float *maxima = reinterpret_cast<volatile float *>(gbase + L::kOffMsg) + row;
+        volatile float2 *ends = reinterpret_cast<volatile float2 *>(gbase + L::kOffEnd) + row;
+        const int pair_bar = 1 + quarter;
         const float c = args.c;
         PromptItem w;
         uint32_t steps = 0;
         int outs = 0;
         bool ok = true;
         for (int seq = 0; ok && (ok = next_item(seq, w)); ++seq) {
-            const int mine = t ? w.n1 : w.n0, r = t * kRows + row;
+            const int mine = w.n, r = row;
             const int see = args.causal ? max(0, min(w.lk, w.see + r)) : w.lk;      // keys that this row sees
             const int all = __shfl_sync(0xffffffffu, see, 0);                       // ... and every row of this warp
             float m = -INFINITY, l = 0.f;      // the reference that this warpgroup's last step was taken with, and its weights' sum
             for (int j = (steps & 1) ^ par; j < mine; j += 2) {
                 const uint32_t step = steps + j;
-                if (!warp_wait(bar(PB_SFULL + t * 2 + par), (step >> 1) & 1, ctl, W + 15)) { ok = false; break; }
+                if (!warp_wait(bar(PB_SFULL + par), (step >> 1) & 1, ctl, W + 15)) { ok = false; break; }
                 tc_fence_after();
-                // The product that read what P overwrites is done (over S that is so, or S could not have been computed).  Before the message:
-                // whoever has that knows which phase of this barrier comes next.
-                if (!L::kOverlay && step > 1) {
-                    if (!warp_wait(bar(PB_PVDONE + t * 2 + par), ((step >> 1) - 1) & 1, ctl, W + 14)) { ok = false; break; }
+                // The product that read what P overwrites is done.  Before the message: whoever has that knows which phase of this barrier comes next.
+                if (step > 1) {
+                    if (!warp_wait(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1, ctl, W + 14)) { ok = false; break; }
                     tc_fence_after();
                 }
                 // what the step before was taken with; every message is waited for before the next one is sent
@@ -473,10 +417,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 }
                 bool with_max = j == 0;
                 float before = ref, sum;
-                uint32_t p[32];
+                uint32_t p[kKeys / 2];
                 while (true) {
                     float s[kKeys];
-                    tmem_ld32x2_sync(tS, tS + 32, reinterpret_cast<uint32_t *>(s), reinterpret_cast<uint32_t *>(s) + 32);
+                    tmem_row(tS, reinterpret_cast<uint32_t *>(s));
                     if (args.negate)
 #pragma unroll
                         for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
@@ -539,12 +483,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     }
                 }
                 if (!ok) break;
-                if (!L::kOverlay) {
-                    tc_fence_before();
-                    warp_arrive(bar(PB_SFREE + t * 2 + par));
-                }
+                tc_fence_before();
+                warp_arrive(bar(PB_SFREE + par));
                 if (with_max && j > 0) {
-                    if (!warp_wait(bar(PB_PVDONE + t * 2 + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17)) { ok = false; break; }
+                    if (!warp_wait(bar(PB_PVDONE + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17)) { ok = false; break; }
                     tc_fence_after();
                     const float keep = before == ref ? 1.f : before == -INFINITY ? 0.f : ex2((before - ref) * c);
 #pragma unroll
@@ -557,16 +499,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     }
                 }
                 tmem_st32(tP, p);
+                tmem_st32(tP + 32, p + 32);
                 tmem_st_wait();
                 tc_fence_before();
-                warp_arrive(bar(PB_PFULL + t * 2 + par));
+                warp_arrive(bar(PB_PFULL + par));
                 l = fmaf(l, m == ref ? 1.f : m == -INFINITY ? 0.f : ex2((m - ref) * c), sum);
                 m = ref;
             }
             steps += mine;
             if (!ok) break;
             // maxima and sums of both warpgroups: the larger maximum is the later one
-            volatile float2 *e = ends + (seq & 1) * 4 * kRows;
+            volatile float2 *e = ends + (seq & 1) * 2 * kRows;
             e[par * kRows].x = m;
             e[par * kRows].y = l;
             named_bar_sync(pair_bar, 64);
@@ -575,7 +518,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             const float ref = top == -INFINITY ? 0.f : top;
             l = l * ex2((m - ref) * c) + l2 * ex2((m2 - ref) * c);
             if (mine > 0) {
-                if (!(ok = warp_wait(bar(PB_OFULL + t), outs++ & 1, ctl, W + 18))) break;
+                if (!(ok = warp_wait(bar(PB_OFULL), outs++ & 1, ctl, W + 18))) break;
                 tc_fence_after();
             }
             const bool none = top == -INFINITY && l < 1e-20f;      // (l is not a number, or not finite, where a score is not a number)
@@ -598,7 +541,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             }
             if (mine > 0) {
                 tc_fence_before();
-                warp_arrive(bar(PB_OFREE + t));
+                warp_arrive(bar(PB_OFREE));
             }
             if (args.lse && mine_row && par == 0)
                 args.lse[(long long)(w.q0 + r) * args.n_q + w.head] = none ? -INFINITY : (top * c + log2f(l)) * 0.6931471805599453f;
@@ -622,16 +565,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 template <int HD>
 int launch_prompt(const flashmhf_prompt_attention_params &p, const PromptArgs &a, int device, cudaStream_t st, int *n_launch) {
     CUtensorMap q, k, v;
-    auto map = [&](CUtensorMap *m, const void *ptr, const int64_t *stride, int heads, int tokens, int rows) {
+    auto map = [&](CUtensorMap *m, const void *ptr, const int64_t *stride, int heads, int tokens) {
         if (tokens == 0) heads = tokens = 1;      // no keys at all: nothing is read through the map
         const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)heads, (uint64_t)tokens};
         const int64_t str[2] = {stride[1], stride[0]};
-        const uint32_t box[3] = {64, 1, (uint32_t)rows};
+        const uint32_t box[3] = {64, 1, kRows};
         return encode_bf16_map(m, ptr, 3, dims, str, box);
     };
-    int rc = map(&q, p.q, p.q_stride, p.n_q, p.tokens_q, kRows);
-    if (rc == FLASHMHF_OK) rc = map(&k, p.k, p.k_stride, p.n_kv, p.tokens_k, kKeys);
-    if (rc == FLASHMHF_OK) rc = map(&v, p.v, p.v_stride, p.n_kv, p.tokens_k, kKeys);
+    int rc = map(&q, p.q, p.q_stride, p.n_q, p.tokens_q);
+    if (rc == FLASHMHF_OK) rc = map(&k, p.k, p.k_stride, p.n_kv, p.tokens_k);
+    if (rc == FLASHMHF_OK) rc = map(&v, p.v, p.v_stride, p.n_kv, p.tokens_k);
     if (rc != FLASHMHF_OK) return rc;
     const size_t smem = PromptCfg<HD>::kTotal;
     cudaError_t e = cudaSuccess;
@@ -657,7 +600,7 @@ int prompt_attention(const flashmhf_prompt_attention_params &p, const DeviceCtl 
     a.o_tok = p.o_stride[0]; a.o_head = p.o_stride[1];
     a.lse = p.lse; a.cu_q = p.cu_q; a.cu_k = p.cu_k;
     a.B = p.B; a.tokens_q = p.tokens_q; a.tokens_k = p.tokens_k; a.n_q = p.n_q; a.group = p.n_q / p.n_kv; a.causal = p.causal != 0;
-    const long long items = ((long long)p.tokens_q / kItemRows + p.B) * p.n_q;
+    const long long items = ((long long)p.tokens_q / kRows + p.B) * p.n_q;
     if (items > 0x3fffffffll) return FLASHMHF_ERR_BAD_SHAPE;
     a.n_items = (int)items;
     a.negate = p.scale < 0.f;
