@@ -35,7 +35,7 @@ namespace {
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 4) * 32;
 constexpr int kKernelPrompt = 6;                  // status codes 601..
-constexpr float kLazy = 65536.f;                  // the sum of a row's weights of a step above which its reference is set anew
+constexpr float kLazy = 16.f;                     // how far (in powers of two) a row's reference may be exceeded before O is scaled to a new one
 constexpr int kLag = 8;
 constexpr int kMaxStages = 4;
 
@@ -393,102 +393,43 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             float m = -INFINITY, l = 0.f;      // the reference that this warpgroup's last step was taken with, and its weights' sum
             for (int j = (steps & 1) ^ par; j < mine; j += 2) {
                 const uint32_t step = steps + j;
-                if (!warp_wait(bar(PB_SFULL + par), (step >> 1) & 1, ctl, W + 15)) { ok = false; break; }
+                if (!warp_wait(bar(PB_SFULL + par), (step >> 1) & 1, ctl, W + 18)) { ok = false; break; }
                 tc_fence_after();
-                // The product that read what P overwrites is done.  Before the message: whoever has that knows which phase of this barrier comes next.
-                if (step > 1) {
-                    if (!warp_wait(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1, ctl, W + 14)) { ok = false; break; }
-                    tc_fence_after();
-                }
-                // what the step before was taken with; every message is waited for before the next one is sent
-                bool heard = step == 0;
-                float ref = m;
-                auto hear = [&]() -> bool {
-                    heard = true;
-                    return warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16);
-                };
-                auto send = [&] {
-                    maxima[par * kRows] = ref;
-                    warp_arrive(msg_out);
-                };
-                if (j == 1) {
-                    if (!hear()) { ok = false; break; }
-                    ref = maxima[(par ^ 1) * kRows];
-                }
-                bool with_max = j == 0;
-                float before = ref, sum;
-                uint32_t p[kKeys / 2];
-                while (true) {
-                    float s[kKeys];
-                    tmem_row(tS, reinterpret_cast<uint32_t *>(s));
-                    if (args.negate)
-#pragma unroll
-                        for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
-                    if ((j + 1) * kKeys > all) {
-                        const int left = see - j * kKeys;
-#pragma unroll
-                        for (int i = 0; i < kKeys; ++i) s[i] = i < left ? s[i] : -INFINITY;
-                    }
-                    if (with_max) {
-                        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                        for (int i = 4; i < kKeys; i += 8)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) top[k] = i + 4 < kKeys ? max3(top[k], s[i + k], s[i + 4 + k]) : fmaxf(top[k], s[i + k]);
-                        before = ref;
-                        ref = fmaxf(ref, fmaxf(max3(top[0], top[1], top[2]), top[3]));
-                        if (!heard && !hear()) { ok = false; break; }
-                        send();          // (no weight of this pass is above 1: it stays)
-                    }
-                    const float mc = ref == -INFINITY ? 0.f : -ref * c;
-                    const f32x2 c2 = f2_pack(c, c), mc2 = f2_pack(mc, mc);
-                    f32x2 sum0 = 0, sum1 = 0;
-#pragma unroll
-                    for (int i = 0; i < kKeys + kLag; i += 8) {
-                        if (i < kKeys) {
-#pragma unroll
-                            for (int k = 0; k < 8; k += 2) {
-                                f2_unpack(f2_fma(f2_pack(s[i + k], s[i + k + 1]), c2, mc2), s[i + k], s[i + k + 1]);
-                                s[i + k] = ex2(s[i + k]);
-                                s[i + k + 1] = ex2(s[i + k + 1]);
-                            }
-                        }
-                        if (i >= kLag) {
-                            const int y = i - kLag;
-#pragma unroll
-                            for (int k = 0; k < 8; k += 4) {
-                                sum0 = f2_add(sum0, f2_pack(s[y + k], s[y + k + 1]));
-                                sum1 = f2_add(sum1, f2_pack(s[y + k + 2], s[y + k + 3]));
-                                p[(y + k) / 2] = pack_bf16(s[y + k], s[y + k + 1]);
-                                p[(y + k) / 2 + 1] = pack_bf16(s[y + k + 2], s[y + k + 3]);
-                            }
-                        }
-                    }
-                    float a0, a1;
-                    f2_unpack(f2_add(sum0, sum1), a0, a1);
-                    sum = a0 + a1;
-                    if (with_max) break;
-                    bool stale = false;
-                    if (!heard) {
-                        if (!hear()) { ok = false; break; }
-                        const float now = maxima[(par ^ 1) * kRows];
-                        stale = now != ref;
-                        ref = now;
-                    }
-                    if (__any_sync(0xffffffffu, stale)) continue;       // the other warpgroup took a new reference: once more with that
-                    with_max = __any_sync(0xffffffffu, sum > kLazy || (ref == -INFINITY && sum > 0.f));
-                    if (!with_max) {
-                        send();
-                        break;
-                    }
-                }
-                if (!ok) break;
+                float s[kKeys];
+                tmem_row(tS, reinterpret_cast<uint32_t *>(s));
                 tc_fence_before();
                 warp_arrive(bar(PB_SFREE + par));
-                if (with_max && j > 0) {
+                // Asked here, needed behind the maximum: is the product done that read what P will overwrite, and has the step before said what it
+                // was taken with?  Both are waited for before this step's own message: whoever has that knows these phases to be over.
+                const bool asked = (step < 2 || mbar_test(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1)) && (step == 0 || mbar_test(msg_in, ((step - 1) >> 1) & 1));
+                if (args.negate)
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
+                if ((j + 1) * kKeys > all) {
+                    const int left = see - j * kKeys;
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) s[i] = i < left ? s[i] : -INFINITY;
+                }
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < kKeys; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = i + 4 < kKeys ? max3(top[k], s[i + k], s[i + 4 + k]) : fmaxf(top[k], s[i + k]);
+                const float x = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+                if (!__all_sync(0xffffffffu, asked) &&
+                    ((step > 1 && !warp_wait(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1, ctl, W + 15)) ||
+                     (step > 0 && !warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16)))) { ok = false; break; }
+                tc_fence_after();
+                const float was = j > 0 ? maxima[(par ^ 1) * kRows] : -INFINITY;
+                // (the first finite maximum of a row is always taken: -inf is exceeded by more than anything)
+                const bool any = __any_sync(0xffffffffu, (x - was) * c > kLazy);
+                const float ref = any ? fmaxf(was, x) : was;
+                maxima[par * kRows] = ref;
+                warp_arrive(msg_out);
+                if (any && j > 0) {
                     if (!warp_wait(bar(PB_PVDONE + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17)) { ok = false; break; }
                     tc_fence_after();
-                    const float keep = before == ref ? 1.f : before == -INFINITY ? 0.f : ex2((before - ref) * c);
+                    const float keep = was == ref ? 1.f : was == -INFINITY ? 0.f : ex2((was - ref) * c);
 #pragma unroll
                     for (int d = 0; d < HD; d += 16) {
                         uint32_t o[16];
@@ -498,12 +439,38 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         tmem_st16(tO + d, o);
                     }
                 }
-                tmem_st32(tP, p);
-                tmem_st32(tP + 32, p + 32);
+                const float mc = ref == -INFINITY ? 0.f : -ref * c;
+                const f32x2 c2 = f2_pack(c, c), mc2 = f2_pack(mc, mc);
+                f32x2 sum0 = 0, sum1 = 0;
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < kKeys + kLag; i += 8) {
+                    if (i < kKeys) {
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2) {
+                            f2_unpack(f2_fma(f2_pack(s[i + k], s[i + k + 1]), c2, mc2), s[i + k], s[i + k + 1]);
+                            s[i + k] = ex2(s[i + k]);
+                            s[i + k + 1] = ex2(s[i + k + 1]);
+                        }
+                    }
+                    if (i >= kLag) {
+                        const int y = i - kLag;
+#pragma unroll
+                        for (int k = 0; k < 8; k += 4) {
+                            sum0 = f2_add(sum0, f2_pack(s[y + k], s[y + k + 1]));
+                            sum1 = f2_add(sum1, f2_pack(s[y + k + 2], s[y + k + 3]));
+                            p[((y + k) & 63) / 2] = pack_bf16(s[y + k], s[y + k + 1]);
+                            p[((y + k) & 63) / 2 + 1] = pack_bf16(s[y + k + 2], s[y + k + 3]);
+                        }
+                        if ((y & 63) == 56) tmem_st32(tP + y / 64 * 32, p);
+                    }
+                }
+                float a0, a1;
+                f2_unpack(f2_add(sum0, sum1), a0, a1);
                 tmem_st_wait();
                 tc_fence_before();
                 warp_arrive(bar(PB_PFULL + par));
-                l = fmaf(l, m == ref ? 1.f : m == -INFINITY ? 0.f : ex2((m - ref) * c), sum);
+                l = fmaf(l, m == ref ? 1.f : m == -INFINITY ? 0.f : ex2((m - ref) * c), a0 + a1);
                 m = ref;
             }
             steps += mine;
@@ -518,7 +485,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             const float ref = top == -INFINITY ? 0.f : top;
             l = l * ex2((m - ref) * c) + l2 * ex2((m2 - ref) * c);
             if (mine > 0) {
-                if (!(ok = warp_wait(bar(PB_OFULL), outs++ & 1, ctl, W + 18))) break;
+                if (!(ok = warp_wait(bar(PB_OFULL), outs++ & 1, ctl, W + 19))) break;
                 tc_fence_after();
             }
             const bool none = top == -INFINITY && l < 1e-20f;      // (l is not a number, or not finite, where a score is not a number)
