@@ -273,17 +273,24 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                             tma_load_3d(sQ + qb * L::kTile + c * L::kChunk, &tmQ, bar(PB_QFULL + qb), c * 64, w.head, w.q0);
                     }
                     const int kh = w.head / args.group;
-                    for (int j = 0; j < n; ++j, ++g) {
-                        const uint32_t st = g % NS, lap = (g / NS) & 1;
-                        if (!thread_wait(bar(PB_KEMPTY + st), lap ^ 1, ctl, W + 4)) { ok = false; break; }
-                        mbar_arrive_expect_tx(bar(PB_KFULL + st), L::kTile);
-                        for (int c = 0; c < L::kChunks; ++c)
-                            tma_load_3d(sK + st * L::kTile + c * L::kChunk, &tmK, bar(PB_KFULL + st), c * 64, kh, w.k0 + j * kKeys);
-                        if (!thread_wait(bar(PB_VEMPTY + st), lap ^ 1, ctl, W + 5)) { ok = false; break; }
-                        const uint32_t full = bar(((j + 1) * kKeys > w.lk ? PB_VRAW : PB_VFULL) + st);
-                        mbar_arrive_expect_tx(full, L::kTile);
-                        for (int c = 0; c < L::kChunks; ++c) tma_load_3d(sV + st * L::kTile + c * L::kChunk, &tmV, full, c * 64, kh, w.k0 + j * kKeys);
+                    // keys of tile j, then values of tile j - 1, which are needed that much later: keys never wait for a stage of values
+                    for (int j = 0; ok && j <= n && n > 0; ++j) {
+                        if (j < n) {
+                            const uint32_t st = (g + j) % NS;
+                            if (!thread_wait(bar(PB_KEMPTY + st), ((g + j) / NS & 1) ^ 1, ctl, W + 4)) { ok = false; break; }
+                            mbar_arrive_expect_tx(bar(PB_KFULL + st), L::kTile);
+                            for (int c = 0; c < L::kChunks; ++c)
+                                tma_load_3d(sK + st * L::kTile + c * L::kChunk, &tmK, bar(PB_KFULL + st), c * 64, kh, w.k0 + j * kKeys);
+                        }
+                        if (j > 0) {
+                            const uint32_t st = (g + j - 1) % NS;
+                            if (!thread_wait(bar(PB_VEMPTY + st), ((g + j - 1) / NS & 1) ^ 1, ctl, W + 5)) { ok = false; break; }
+                            const uint32_t full = bar((j * kKeys > w.lk ? PB_VRAW : PB_VFULL) + st);
+                            mbar_arrive_expect_tx(full, L::kTile);
+                            for (int c = 0; c < L::kChunks; ++c) tma_load_3d(sV + st * L::kTile + c * L::kChunk, &tmV, full, c * 64, kh, w.k0 + (j - 1) * kKeys);
+                        }
                     }
+                    g += n;
                     if (!ok || !thread_wait(bar(PB_NEXT), asked++ & 1, ctl, W + 6)) break;
                     uint32_t got, next;
                     asm volatile(
