@@ -1,28 +1,30 @@
 // Attention over packed prompts, bf16, sm_100a:  O = softmax(scale Q K^T + mask) V  per sequence and query head.
 //
-// A work item is 256 consecutive rows of one sequence and query head, in two tiles of 128 rows; both read the same tiles of 64 keys.  Per tile
-// of keys and tile of rows the tensor core computes S = Q K^T (128 x 64, fp32 in tensor memory), one warpgroup (a thread a row) takes the
-// running maximum and P = bf16(2^(c s - c m)) and writes it over S, and the tensor core adds P V to O (fp32, in tensor memory over all
-// keys): scores and weights never leave the SM.
+// A work item is a tile of 128 consecutive rows of one sequence and query head; it walks over its keys 128 at a time.  A step: the tensor
+// core computes S = Q K^T (128 x 128, fp32 in tensor memory), a warpgroup (a thread a row) takes P = bf16(2^(c s - c r)), r a reference
+// of the row near its maximum, into tensor memory, and the tensor core adds P V to O (fp32, in tensor memory over all steps): scores and
+// weights never leave the SM.
 //
-// Bound: latencies first, exponentials second.  The special function units take 512 clk for 128 x 64 exponentials, the products 370 (a head of 64) to
-// 650 clk (128); but from S to P a step is a chain of some 1800 clk (barriers, tensor memory both ways, the maximum, a warp's exponentials).
-// So four chains are under way: each tile of rows has two buffers of S and two warpgroups, which take its steps in turn.  A step needs
-// nothing of the one before but its maximum, which is known early and goes through shared memory.
+// Bound: a chain of latencies, then the exponentials, then the way from L2.  The special function units take 1024 clk for the 128 x 128
+// exponentials of a step and the two products 620 (a head of 64) to 1030 clk (128), but from S to P a step takes a warp some 3500 clk: tensor memory
+// both ways, the maximum, barriers, and exponentials which a warp alone asks for at 68 % of the units' rate.  So two warpgroups take the
+// steps in turn, with S and P in two buffers each.  Measured: 1770 (64) and 2000 clk (128) a step, special function units 53 % busy, tensor pipe 26
+// and 50 %; 8192 causal tokens of 32 heads of 128 at 1.16 PFLOP/s (474 us), 1.0 in a loop at the power limit.  What did not help: two tiles
+// of rows a block (half the keys from L2, but tensor memory then has P only over S, and S waits for the product that reads P: 522 against 475 us with
+// two warpgroups a tile), three warpgroups (the same reason: 547), four with 64 keys (a step costs each issuing thread 1000 clk whatever
+// its size: 581), a cubic on the FMA pipe for a quarter of the exponentials (the same time), items in the order of their length and handed out one
+// ahead (the order costs more than it gives: 56 -> 59 us for twelve ragged prompts, 139 -> 197 for 64 short ones).
 //
-// The maximum is lazy: O is multiplied by 2^(c m_old - c m_new) only where a new maximum is more than 2^8 above the one in use (P is then
-// at most 256, and P, its sum and O are all in one scale), so that almost no step touches O.
-//
-// No product writes tensor memory that another one may still be reading on the strength of the order of issue alone (that order is promised for
-// products of one accumulator and shape).  A head of 64 leaves room for P beside S; with heads of 96 and 128 P lies over S, and S of step s + 2
-// waits until the product that reads P of step s is done.
+// The reference is lazy: it is set to the maximum so far only where a row exceeds it by more than 2^16, and O is then multiplied by 2^(c r_old -
+// c r_new).  P, its sum and O hold such values without loss (bf16 and fp32 are relative), so that almost no step touches O.  A step hands
+// its reference on to the next one, in the other warpgroup, through shared memory.
 //
 // Work items are handed out by the hardware: the grid has a block for each, a resident block takes over one that has not started
 // (clusterlaunchcontrol) while it works on its own.
 //
-// Warp roles: 0-15 softmax (tile of rows = warp / 8, parity of the steps = warp / 4 % 2, TMEM lane quarter = warp % 4), 16 work items and TMA, 17
-// issues S of both tiles, 18 and 19 O += P V of one each; 18 also clears the rows of V behind the end of a sequence (a weight of 0 does not undo a
-// NaN of the next one).
+// Warp roles: 0-3 and 4-7 softmax of the even and the odd steps (warp % 4 = TMEM lane quarter = 32 rows), 8 work items and TMA, 9 issues S, 10 O
+// += P V and clears the rows of V behind the end of a sequence (a weight of 0 does not undo a NaN of the next one), 12-15 write out an item's rows
+// while the others are at the next.
 #include <atomic>
 
 #include "paged.cuh"
@@ -33,7 +35,7 @@ namespace fmhf {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128;
-constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 4) * 32;
+constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 8) * 32;
 constexpr int kKernelPrompt = 6;                  // status codes 601..
 constexpr float kLazy = 16.f;                     // how far (in powers of two) a row's reference may be exceeded before O is scaled to a new one
 constexpr int kLag = 8;
@@ -47,19 +49,22 @@ struct PromptCfg {
     static constexpr uint32_t kTile = kChunks * kChunk;
     static constexpr uint32_t kOffQ = 0, kOffK = 2 * kTile, kOffV = kOffK + kStages * kTile;
     static constexpr uint32_t kOffMsg = kOffV + kStages * kTile, kOffEnd = kOffMsg + 2 * kRows * 4;   // [parity][row]: references; those and sums (of two items)
-    static constexpr uint32_t kOffBar = kOffEnd + 2 * 2 * kRows * 8, kTotal = kOffBar + 512 + 1024;
+    static constexpr uint32_t kOffBar = kOffEnd + 2 * 2 * kRows * 8, kTotal = kOffBar + 640 + 1024;
 };
-// Tensor memory: two buffers for S, two for P (two bf16 a column), O.
+// Tensor memory: two buffers for S, two for P (two bf16 a column), one for O, or two where there is room.
 constexpr uint32_t kColP = 256, kColO = 384;
+template <int HD>
+constexpr int kOBufs = HD == 64 ? 2 : 1;
 
 // SFULL: S computed into a buffer; SFREE: it is in registers; PFULL: P written, O scaled if need be; PVDONE: the product that read P is done (+
-// buffer); OFULL: the last one of an item; OFREE: O has been read out; MSG: the reference that a step was taken with (quarter q, steps of parity
-// b: + 2 q + b); ITEM*: the ring of work items; NEXT: the answer to a request for one.
-enum { PB_QFULL = 0, PB_QEMPTY = 2, PB_SFULL = 4, PB_SFREE = 6, PB_PFULL = 8, PB_PVDONE = 10, PB_OFULL = 12, PB_OFREE = 13, PB_ITEMFULL = 14,
-       PB_ITEMEMPTY = 16, PB_NEXT = 18, PB_MSG = 19, PB_KFULL = 27, PB_KEMPTY = PB_KFULL + kMaxStages, PB_VFULL = PB_KEMPTY + kMaxStages,
-       PB_VEMPTY = PB_VFULL + kMaxStages, PB_VRAW = PB_VEMPTY + kMaxStages, PB_COUNT = PB_VRAW + kMaxStages };
+// buffer); OFULL: the last one of an item; OFREE: O has been read out (+ buffer); MSG: the reference that a step was taken with (quarter q, steps
+// of parity b: + 2 q + b); ENDS, ENDSFREE: references and sums of an item's rows written, read; ITEM*: the ring of work items; NEXT: the answer
+// to a request for one.
+enum { PB_QFULL = 0, PB_QEMPTY = 2, PB_SFULL = 4, PB_SFREE = 6, PB_PFULL = 8, PB_PVDONE = 10, PB_OFULL = 12, PB_OFREE = 14, PB_ITEMFULL = 16,
+       PB_ITEMEMPTY = 18, PB_ENDS = 20, PB_ENDSFREE = 22, PB_NEXT = 24, PB_MSG = 25, PB_KFULL = 33, PB_KEMPTY = PB_KFULL + kMaxStages,
+       PB_VFULL = PB_KEMPTY + kMaxStages, PB_VEMPTY = PB_VFULL + kMaxStages, PB_VRAW = PB_VEMPTY + kMaxStages, PB_COUNT = PB_VRAW + kMaxStages };
 constexpr uint32_t kOffNext = (PB_COUNT * 8 + 15) / 16 * 16, kOffItems = kOffNext + 16, kOffCtl = kOffItems + 2 * 48;
-static_assert(kOffCtl + 8 <= 512, "control area");
+static_assert(kOffCtl + 8 <= 640, "control area");
 
 struct PromptItem {
     int q0, lq;          // first row of the item in the packed rows; rows of the sequence from there on
@@ -183,7 +188,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     auto bar = [&](int i) { return sBar + 8u * i; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtl ctl{abort_flag, args.wait};
-    constexpr int W = kKernelPrompt * 100, kLoad = kSoftmaxWarps, kIssue = kLoad + 1;
+    constexpr int W = kKernelPrompt * 100, kLoad = kSoftmaxWarps, kIssue = kLoad + 1, kOut = kLoad + 4;
 
     if (threadIdx.x == 0) {
         *abort_flag = launch_aborted(args.wait);
@@ -195,10 +200,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             mbar_init(bar(PB_PFULL + i), 4);
             mbar_init(bar(PB_PVDONE + i), 1);
             mbar_init(bar(PB_ITEMFULL + i), 1);
-            mbar_init(bar(PB_ITEMEMPTY + i), kSoftmaxWarps + 2);      // every warp but the one that fills it
+            mbar_init(bar(PB_OFULL + i), 1);
+            mbar_init(bar(PB_OFREE + i), 4);
+            mbar_init(bar(PB_ENDS + i), kSoftmaxWarps);
+            mbar_init(bar(PB_ENDSFREE + i), 4);
+            mbar_init(bar(PB_ITEMEMPTY + i), kSoftmaxWarps + 6);      // softmax, both issuers, output
         }
-        mbar_init(bar(PB_OFULL), 1);
-        mbar_init(bar(PB_OFREE), 8);
         for (int i = 0; i < 8; ++i) mbar_init(bar(PB_MSG + i), 1);
         mbar_init(bar(PB_NEXT), 1);
         for (int i = 0; i < NS; ++i) {
@@ -230,9 +237,53 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 
     if (*abort_flag) {
         // nothing: fall through to the teardown
+    } else if (warp >= kOut) {
+        // ------------------------------------------------------------------ output, a thread a row, while the other warps are at the next item
+        // (registers: 256 x 208 for rows of S + 256 x 48 are the 512 x 128 that the launch has)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        const int row = (warp & 3) * 32 + lane;
+        PromptItem w;
+        int outs = 0;
+        for (int seq = 0; next_item(seq, w); ++seq) {
+            if (!warp_wait(bar(PB_ENDS + (seq & 1)), (seq >> 1) & 1, ctl, W + 20)) break;
+            // references and sums of both warpgroups: the larger reference is the later one
+            volatile float2 *e = reinterpret_cast<volatile float2 *>(gbase + L::kOffEnd) + (seq & 1) * 2 * kRows + row;
+            const float m0 = e[0].x, l0 = e[0].y, m1 = e[kRows].x, l1 = e[kRows].y, top = fmaxf(m0, m1), ref = top == -INFINITY ? 0.f : top;
+            warp_arrive(bar(PB_ENDSFREE + (seq & 1)));
+            const float l = l0 * ex2((m0 - ref) * args.c) + l1 * ex2((m1 - ref) * args.c);
+            const bool none = top == -INFINITY && l < 1e-20f;      // (l is not a number, or not finite, where a score is not a number)
+            const float inv = 1.f / l;
+            const bool in = row < w.lq;
+            const int ob = outs % kOBufs<HD>;
+            const uint32_t tO = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kColO + ob * 64;
+            if (w.n > 0) {
+                if (!warp_wait(bar(PB_OFULL + ob), (outs / kOBufs<HD>) & 1, ctl, W + 19)) break;
+                tc_fence_after();
+                ++outs;
+            }
+            __nv_bfloat16 *dst = args.o + (long long)(w.q0 + row) * args.o_tok + (long long)w.head * args.o_head;
+#pragma unroll
+            for (int d = 0; d < HD; d += 16) {
+                uint32_t o[16] = {};
+                if (w.n > 0) tmem_ld16_sync(tO + d, o);
+                if (in)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            v[k] = none ? 0u : pack_bf16(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+                        *reinterpret_cast<uint4 *>(dst + d + i) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+            }
+            if (w.n > 0) {
+                tc_fence_before();
+                warp_arrive(bar(PB_OFREE + ob));
+            }
+            if (args.lse && in) args.lse[(long long)(w.q0 + row) * args.n_q + w.head] = none ? -INFINITY : (top * args.c + log2f(l)) * 0.6931471805599453f;
+        }
     } else if (warp >= kSoftmaxWarps) {
-        // A softmax thread holds a row of S: 256 x 208 + 128 x 88 registers, the 384 x 168 that the launch has.
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == kLoad) {
             // -------------------------------------------------------------- work items and TMA
             if (lane == 0) {
@@ -348,6 +399,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             int outs = 0;
             bool ok = true;
             for (int seq = 0; ok && next_item(seq, w); ++seq) {
+                const int ob = outs % kOBufs<HD>;
                 for (int j = 0; j < w.n; ++j, ++s) {
                     const uint32_t st = s % NS, b = s & 1;
                     if ((j + 1) * kKeys > w.lk) {
@@ -360,17 +412,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         warp_arrive(bar(PB_VFULL + st));
                     }
                     if (!warp_wait(bar(PB_VFULL + st), (s / NS) & 1, ctl, W + 12)) { ok = false; break; }
-                    if (j == 0 && outs > 0 && !warp_wait(bar(PB_OFREE), (outs - 1) & 1, ctl, W + 13)) { ok = false; break; }
+                    if (j == 0 && outs >= kOBufs<HD> && !warp_wait(bar(PB_OFREE + ob), (outs / kOBufs<HD> - 1) & 1, ctl, W + 13)) { ok = false; break; }
                     if (!warp_wait(bar(PB_PFULL + b), (s >> 1) & 1, ctl, W + 14)) { ok = false; break; }
                     tc_fence_after();
                     if (lane == 0) {
 #pragma unroll
                         for (int k = 0; k < kKeys / 16; ++k)
-                            umma_ts(tmem + kColO, tmem + kColP + b * (kKeys / 2) + k * 8, dV0 + st * (L::kTile >> 4) + k * 128, idesc,
+                            umma_ts(tmem + kColO + ob * 64, tmem + kColP + b * (kKeys / 2) + k * 8, dV0 + st * (L::kTile >> 4) + k * 128, idesc,
                                     (j > 0 || k > 0) ? 1u : 0u);
                         umma_commit(bar(PB_PVDONE + b));
                         umma_commit(bar(PB_VEMPTY + st));
-                        if (j + 1 == w.n) umma_commit(bar(PB_OFULL));
+                        if (j + 1 == w.n) umma_commit(bar(PB_OFULL + ob));
                     }
                     __syncwarp();
                 }
@@ -378,24 +430,23 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             }
         }
     } else {
-        // ------------------------------------------------------------------ softmax and output, a thread a row
+        // ------------------------------------------------------------------ softmax, a thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        constexpr int NO = HD / 2;                   // columns of O that each of the two warpgroups of a tile writes out
         const int par = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t tS = lanes + par * kKeys, tP = lanes + kColP + par * (kKeys / 2), tO = lanes + kColO;
+        const uint32_t tS = lanes + par * kKeys, tP = lanes + kColP + par * (kKeys / 2);
         const uint32_t msg_out = bar(PB_MSG + 2 * quarter + par), msg_in = bar(PB_MSG + 2 * quarter + (par ^ 1));
-        volatile float *maxima = reinterpret_cast<volatile float *>(gbase + L::kOffMsg) + row;
-        volatile float2 *ends = reinterpret_cast<volatile float2 *>(gbase + L::kOffEnd) + row;
-        const int pair_bar = 1 + quarter;
+        volatile float *refs = reinterpret_cast<volatile float *>(gbase + L::kOffMsg) + row;
+        volatile float2 *ends = reinterpret_cast<volatile float2 *>(gbase + L::kOffEnd) + par * kRows + row;
         const float c = args.c;
         PromptItem w;
         uint32_t steps = 0;
         int outs = 0;
         bool ok = true;
         for (int seq = 0; ok && (ok = next_item(seq, w)); ++seq) {
-            const int mine = w.n, r = row;
-            const int see = args.causal ? max(0, min(w.lk, w.see + r)) : w.lk;      // keys that this row sees
+            const int mine = w.n;
+            const uint32_t tO = lanes + kColO + outs % kOBufs<HD> * 64;
+            const int see = args.causal ? max(0, min(w.lk, w.see + row)) : w.lk;      // keys that this row sees
             const int all = __shfl_sync(0xffffffffu, see, 0);                       // ... and every row of this warp
             float m = -INFINITY, l = 0.f;      // the reference that this warpgroup's last step was taken with, and its weights' sum
             for (int j = (steps & 1) ^ par; j < mine; j += 2) {
@@ -406,9 +457,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 tmem_row(tS, reinterpret_cast<uint32_t *>(s));
                 tc_fence_before();
                 warp_arrive(bar(PB_SFREE + par));
-                // Asked here, needed behind the maximum: is the product done that read what P will overwrite, and has the step before said what it
-                // was taken with?  Both are waited for before this step's own message: whoever has that knows these phases to be over.
-                const bool asked = (step < 2 || mbar_test(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1)) && (step == 0 || mbar_test(msg_in, ((step - 1) >> 1) & 1));
+                // Asked here, needed behind the maximum: has the step before said what it was taken with?
+                const bool heard = step == 0 || mbar_test(msg_in, ((step - 1) >> 1) & 1);
                 if (args.negate)
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
@@ -423,18 +473,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
                     for (int k = 0; k < 4; ++k) top[k] = i + 4 < kKeys ? max3(top[k], s[i + k], s[i + 4 + k]) : fmaxf(top[k], s[i + k]);
                 const float x = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-                if (!__all_sync(0xffffffffu, asked) &&
-                    ((step > 1 && !warp_wait(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1, ctl, W + 15)) ||
-                     (step > 0 && !warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16)))) { ok = false; break; }
-                tc_fence_after();
-                const float was = j > 0 ? maxima[(par ^ 1) * kRows] : -INFINITY;
+                if (!__all_sync(0xffffffffu, heard) && !warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16)) { ok = false; break; }
+                const float was = j > 0 ? refs[(par ^ 1) * kRows] : -INFINITY;
                 // (the first finite maximum of a row is always taken: -inf is exceeded by more than anything)
                 const bool any = __any_sync(0xffffffffu, (x - was) * c > kLazy);
                 const float ref = any ? fmaxf(was, x) : was;
-                maxima[par * kRows] = ref;
+                refs[par * kRows] = ref;
                 warp_arrive(msg_out);
                 if (any && j > 0) {
-                    if (!warp_wait(bar(PB_PVDONE + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17)) { ok = false; break; }
+                    // O is complete up to the step before.  One bit of parity tells a phase from the next one only: the product of two steps before
+                    // is done, so P of three steps before has been written, so the next P of that parity is the one that is waited for; and who
+                    // wrote that had waited for the product of three steps before.
+                    if ((step > 1 && !warp_wait(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1, ctl, W + 15)) ||
+                        !warp_wait(bar(PB_PFULL + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17) ||
+                        !warp_wait(bar(PB_PVDONE + (par ^ 1)), ((step - 1) >> 1) & 1, ctl, W + 17)) { ok = false; break; }
                     tc_fence_after();
                     const float keep = was == ref ? 1.f : was == -INFINITY ? 0.f : ex2((was - ref) * c);
 #pragma unroll
@@ -469,9 +521,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                             p[((y + k) & 63) / 2] = pack_bf16(s[y + k], s[y + k + 1]);
                             p[((y + k) & 63) / 2 + 1] = pack_bf16(s[y + k + 2], s[y + k + 3]);
                         }
+                        if (y == 56 && step > 1) {       // the product that read what P overwrites is done
+                            ok = warp_wait(bar(PB_PVDONE + par), ((step >> 1) - 1) & 1, ctl, W + 15);
+                            tc_fence_after();
+                        }
                         if ((y & 63) == 56) tmem_st32(tP + y / 64 * 32, p);
                     }
                 }
+                if (!ok) break;
                 float a0, a1;
                 f2_unpack(f2_add(sum0, sum1), a0, a1);
                 tmem_st_wait();
@@ -481,47 +538,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 m = ref;
             }
             steps += mine;
-            if (!ok) break;
-            // maxima and sums of both warpgroups: the larger maximum is the later one
+            outs += mine > 0;
+            if (!ok || (seq >= 2 && !(ok = warp_wait(bar(PB_ENDSFREE + (seq & 1)), ((seq >> 1) - 1) & 1, ctl, W + 21)))) break;
             volatile float2 *e = ends + (seq & 1) * 2 * kRows;
-            e[par * kRows].x = m;
-            e[par * kRows].y = l;
-            named_bar_sync(pair_bar, 64);
-            if (*abort_flag) { ok = false; break; }      // (set before a warp that gives up arrives here for the last time, below)
-            const float m2 = e[(par ^ 1) * kRows].x, l2 = e[(par ^ 1) * kRows].y, top = fmaxf(m, m2);
-            const float ref = top == -INFINITY ? 0.f : top;
-            l = l * ex2((m - ref) * c) + l2 * ex2((m2 - ref) * c);
-            if (mine > 0) {
-                if (!(ok = warp_wait(bar(PB_OFULL), outs++ & 1, ctl, W + 19))) break;
-                tc_fence_after();
-            }
-            const bool none = top == -INFINITY && l < 1e-20f;      // (l is not a number, or not finite, where a score is not a number)
-            const float inv = 1.f / l;
-            const bool mine_row = r < w.lq;
-            __nv_bfloat16 *dst = args.o + (long long)(w.q0 + r) * args.o_tok + (long long)w.head * args.o_head + par * NO;
-#pragma unroll
-            for (int d = 0; d < NO; d += 16) {
-                uint32_t o[16] = {};
-                if (mine > 0) tmem_ld16_sync(tO + par * NO + d, o);
-                if (mine_row)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            v[k] = none ? 0u : pack_bf16(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
-                        *reinterpret_cast<uint4 *>(dst + d + i) = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
-            }
-            if (mine > 0) {
-                tc_fence_before();
-                warp_arrive(bar(PB_OFREE));
-            }
-            if (args.lse && mine_row && par == 0)
-                args.lse[(long long)(w.q0 + r) * args.n_q + w.head] = none ? -INFINITY : (top * c + log2f(l)) * 0.6931471805599453f;
+            e->x = m;
+            e->y = l;
+            warp_arrive(bar(PB_ENDS + (seq & 1)));
         }
-        // (the warp with the other steps must not wait for this one; if this one gave up, it gives up at its next wait)
-        asm volatile("bar.arrive %0, 64;" ::"r"(pair_bar) : "memory");
     }
     __syncwarp();
     if (*abort_flag) {

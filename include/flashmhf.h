@@ -334,7 +334,8 @@ int flashmhf_paged_attention(const flashmhf_paged_attention_params *p, void *str
 
 /* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1]-1 of q attend to rows cu_k[b] .. cu_k[b+1]-1 of k and v; causal: row r of
  * the lq rows sees key c of the lk keys where c <= r + lk - lq.  A row that sees nothing gives zeros (and -inf); rows of no sequence
- * are left as they are.  lse, if not NULL, fp32 [tokens_q][n_q] contiguous. */
+ * are left as they are.  lse, if not NULL, fp32 [tokens_q][n_q] contiguous.  What the causal mask hides has a weight of zero: a value that is
+ * not a finite number still reaches up to 127 rows before its own, of the same sequence. */
 typedef struct flashmhf_prompt_attention_params {
     const void *q, *k, *v;            /* bf16 [tokens_q | tokens_k][n_q | n_kv][head_dim], innermost contiguous, 16-byte aligned */
     void *o;                          /* bf16 [tokens_q][n_q][head_dim] */
