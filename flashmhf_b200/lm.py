@@ -6,7 +6,8 @@ rotary tables :164-175, FFN layer :256-431, model :784-921, LM head :1055-1090),
 state dict loads with ``load_state_dict``.  The FFN layer is this package's code (the fused prologue + the
 CUDA operator), and on CUDA bf16 tensors the rotary embedding and the hidden-size RMSNorm run through two small
 kernels of the same library (lm_ops.py); attention, projections, embeddings and the loss are plain PyTorch
-calls: they are the surroundings the operator is measured in, not part of it.
+calls: they are the surroundings the operator is measured in, not part of it.  Serving with a paged 8-bit cache
+(PagedKVCache, prefill_paged, decode_step_paged) runs its attention through the library too (serving.py).
 
 ``ffn`` lets a caller substitute the FFN layer function; the default is the CUDA layer and there is
 no CPU stand-in for it in this package.
@@ -202,6 +203,16 @@ class Attention(nn.Module):
             o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=self.nkv != self.nh)
         return self.o_proj(o.transpose(1, 2).reshape(B, S, self.nh * self.hd))
 
+    def paged(self, x, pages, cache, lengths, cu=None):
+        """New tokens of the sequences of a PagedKVCache, whose pages of this layer are ``pages``: x [.., hidden] holds them packed.  With
+        ``cu`` whole prompts (int32 [B+1], their starts): attention over the prompts themselves.  Without, one token a sequence: attention over
+        the pages, of which ``lengths`` (int32 [B]) counts the new token too.  Either way the tokens' keys and values go into the pages."""
+        from . import serving
+        q, k, v = (p(x).view(-1, n, self.hd) for p, n in ((self.q_proj, self.nh), (self.k_proj, self.nkv), (self.v_proj, self.nkv)))
+        q, k = serving.paged_append(pages, k, v, cache.cos, cache.sin, cache.lengths, cache.table, q=q, cu_seqlens=cu, rotated_keys=cu is not None)
+        o = serving.prompt_attention(q, k, v, cu) if cu is not None else serving.paged_attention(q, pages, lengths, cache.table)
+        return self.o_proj(o.view(*x.shape[:-1], self.nh * self.hd))
+
     def decode(self, x, cos_p, sin_p, k_cache, v_cache, pos):
         """One new token per sequence: x [B,1,hidden] at position ``pos`` (a Python int: the same for every sequence),
         rotary tables of that position [1, hd]; appends this token's key and value to the layer's cache at ``pos`` and
@@ -272,6 +283,12 @@ class DecoderLayer(nn.Module):
         that every addition happens in the norm that follows it, across layers too."""
         h, x = add_norm(self.input_layernorm, h, d)
         h, x = add_norm(self.post_attention_layernorm, h, self.self_attn(x, cos, sin, kv_out, link, tables))
+        return h, self.mlp(x)
+
+    def paged(self, h, d, pages, cache, lengths, cu=None):
+        """The layer on h + d with a paged cache (see ``step`` and Attention.paged); returns the new pair."""
+        h, x = add_norm(self.input_layernorm, h, d)
+        h, x = add_norm(self.post_attention_layernorm, h, self.self_attn.paged(x, pages, cache, lengths, cu))
         return h, self.mlp(x)
 
     def decode(self, h, cos_p, sin_p, k_cache, v_cache, pos):
@@ -349,6 +366,66 @@ class KVCache:
         return 2 * L * B * n * length * hd * self.k.element_size()
 
 
+class PagedKVCache:
+    """Keys (rotated) and values of every layer in pages shared by ``batch`` sequences of their own lengths, held in 8 bits
+    (serving.KVPages: half the bytes of KVCache, and none for positions that no sequence has).
+
+    ``lengths`` int32 [batch] (-1: no sequence), ``table`` int32 [batch, max_pages] and the rotary tables live on the device, at addresses that
+    stay, so that a captured ``decode_step_paged`` follows them; who owns which page is kept on the host.  A sequence begins with
+    ``DecoderLM.prefill_paged`` and ends with ``release``; ``reserve`` hands out pages (the two model calls do it themselves, a caller that replays
+    a captured step calls ``reserve`` before and ``advance`` after each)."""
+
+    def __init__(self, cfg, batch, num_pages, page_size=64, max_len=None, device="cuda", dtype=torch.bfloat16):
+        from . import lm_ops, serving
+        hd = cfg.hidden_size // cfg.num_attention_heads
+        self.page_size, self.max_len = page_size, num_pages * page_size if max_len is None else max_len
+        self.pools = [serving.KVPages.empty(num_pages, cfg.num_key_value_heads, page_size, hd, device) for _ in range(cfg.num_hidden_layers)]
+        self.lengths = torch.full((batch,), -1, dtype=torch.int32, device=device)
+        self.table = torch.full((batch, -(-self.max_len // page_size)), -1, dtype=torch.int32, device=device)
+        self.cos, self.sin = lm_ops.rotary_tables_f32(*rotary_tables(self.max_len, hd, cfg.rope_theta, self.lengths.device, dtype))
+        self.held = [-1] * batch                     # tokens of each sequence, as the host knows them
+        self.owned = [[] for _ in range(batch)]      # its pages, in order
+        self.free = list(range(num_pages))[::-1]
+
+    def reserve(self, counts):
+        """Pages for ``counts`` (an int for all sequences, or one each; none for -1) more tokens.  RuntimeError, and nothing changes, where there are
+        not enough pages or a sequence would outgrow ``max_len``."""
+        counts = [counts if n >= 0 else 0 for n in self.held] if isinstance(counts, int) else counts
+        need = []
+        for b, n in enumerate(counts):
+            total = max(self.held[b], 0) + n
+            if total > self.max_len:
+                raise RuntimeError(f"sequence {b}: {total} tokens are more than the cache's max_len {self.max_len}")
+            need.append(-(-total // self.page_size) - len(self.owned[b]))
+        if sum(max(n, 0) for n in need) > len(self.free):
+            raise RuntimeError(f"the cache has {len(self.free)} free pages, {sum(max(n, 0) for n in need)} are needed")
+        rows, cols, vals = [], [], []
+        for b, n in enumerate(need):
+            for _ in range(n):
+                rows.append(b), cols.append(len(self.owned[b])), vals.append(self.free[-1])
+                self.owned[b].append(self.free.pop())
+        if rows:
+            at = torch.tensor([rows, cols, vals], device=self.table.device)
+            self.table[at[0], at[1]] = at[2].int()
+
+    def advance(self, counts):
+        """The host's count of tokens, after ``counts`` more are in the cache."""
+        for b, n in enumerate([counts] * len(self.held) if isinstance(counts, int) else counts):
+            if self.held[b] >= 0:
+                self.held[b] += n
+
+    def release(self, b):
+        """Sequence ``b`` ends: its pages may go to others."""
+        self.free += self.owned[b][::-1]
+        self.owned[b], self.held[b] = [], -1
+        self.lengths[b] = -1
+
+    def nbytes(self):
+        """Bytes of keys, values and scales that a step over what the cache holds reads."""
+        k = self.pools[0].k
+        return len(self.pools) * sum(2 * k.shape[1] * (n * k.shape[3] + 4 * -(-n // self.page_size)) for n in self.held if n > 0)
+
+
 class DecoderLM(nn.Module):
     """ids [B,S] -> logits [B,S,vocab]; ``loss`` is the next-token cross entropy the reference trains with
     (labels = ids shifted by one, mean over B*(S-1) positions, computed in fp32)."""
@@ -416,6 +493,54 @@ class DecoderLM(nn.Module):
         for i, layer in enumerate(self.model.layers):
             h = layer.decode(h, cos_p, sin_p, cache.k[i], cache.v[i], pos)
         return self.lm_head(self.model.norm(h)[:, 0])
+
+    def _paged(self, ids, cache, lengths, cu=None):
+        h, d = self.model.embed_tokens(ids), None
+        for layer, pages in zip(self.model.layers, cache.pools):
+            h, d = layer.paged(h, d, pages, cache, lengths, cu)
+        return add_norm(self.model.norm, h, d)[1]
+
+    @torch.no_grad()
+    def prefill_paged(self, prompts, cache):
+        """Begins sequences in a PagedKVCache: ``prompts`` maps a free place of the batch to its prompt (a 1-D tensor of ids), all of them packed
+        into one pass whatever their lengths.  Returns the logits [len(prompts), vocab] for the token after each, in that order of places."""
+        places = sorted(prompts)
+        for b in places:
+            if cache.held[b] >= 0:
+                raise ValueError(f"place {b} of the cache holds a sequence: release it first")
+            if prompts[b].dim() != 1 or prompts[b].numel() == 0:
+                raise ValueError("a prompt is a 1-D tensor of at least one id")
+        counts = [prompts[b].numel() if b in prompts else 0 for b in range(len(cache.held))]
+        cache.reserve(counts)
+        device = cache.table.device
+        starts = [0]
+        for n in counts:
+            starts.append(starts[-1] + n)
+        cu = torch.tensor(starts, dtype=torch.int32, device=device)
+        at = torch.tensor(places, device=device)
+        cache.lengths[at] = 0
+        for b in places:
+            cache.held[b] = 0
+        ids = torch.cat([prompts[b].to(device) for b in places])
+        h = self._paged(ids[None], cache, None, cu)[0]
+        new = torch.tensor(counts, dtype=torch.int32, device=device)
+        cache.lengths[at] = new[at]
+        cache.advance(counts)
+        return self.lm_head(h[cu[1:][at].long() - 1])
+
+    @torch.no_grad()
+    def decode_step_paged(self, ids, cache):
+        """One token more for every sequence of a PagedKVCache: ids [batch] (of a place without a sequence: any).  Returns the logits [batch, vocab]
+        for the token after it.  Captured into a CUDA graph only the device's part is recorded (see PagedKVCache)."""
+        host = not (ids.is_cuda and torch.cuda.is_current_stream_capturing())
+        if host:
+            cache.reserve(1)
+        lengths = cache.lengths + (cache.lengths >= 0)
+        h = self._paged(ids[:, None], cache, lengths)
+        cache.lengths.copy_(lengths)
+        if host:
+            cache.advance(1)
+        return self.lm_head(h[:, 0])
 
     def forward(self, ids):
         return self.lm_head(self.hidden(ids))
