@@ -6,8 +6,12 @@
 //
 // Splitting.  The tokens of all (sequence, key/value head, eight query rows) are laid end to end in units of 64 and dealt out to all warps of the
 // GPU in equal contiguous runs, by lengths that only the device knows: one long sequence and a hundred short ones load the machine alike.
-// A warp works alone: its codes come by bulk copies into a ring of its own in shared memory (12 KB a warp, 192 KB in flight on an SM: what
-// 6.5 TB/s at over a microsecond's latency take; with the next 16 tokens in registers it was a third less), and go from there into fragments.
+// A warp works alone: its codes come by bulk copies into a ring of its own in shared memory (16 KB a warp, 192 KB on an SM: what 6.5 TB/s at
+// over a microsecond's latency take), and go from there into fragments, 32 tokens at a time: two chains of products, one look at the
+// maximum.  64 sequences of 8192 tokens, 8 heads of 128 (1.07 GB): 185 us = 5.8 TB/s; 64 of 4096, 32 heads of 64: 176 us; two of 65537, 4 heads of
+// 128: 39 us.  In registers, 16 tokens ahead: 224, -, 61.  Sixteen warps with 12 KB and 16 tokens at a time: 179, 203, 43; eight with 24 KB: 188,
+// 204, 38, and 25 instead of 21 us for 32 ragged sequences.  Copies that run on into the next segment of a run: 187, 213, 45 (more instructions a stage
+// than the waits that they save).
 // A run that covers all of an item writes its rows; else the warp writes its part (at most two a warp: the ends of its run) with its maximum
 // and sum, and a second kernel adds the parts in the order of the tokens.
 //
@@ -28,11 +32,10 @@ namespace {
 constexpr int kUnit = 64;            // tokens
 constexpr int kCols = 8;             // query rows of an item
 constexpr int kWarps = 4;            // of a block; they have nothing to do with one another
-constexpr int kBlocksPerSm = 4;
 constexpr int kKernelPaged = 7;      // status codes 701..
 template <int HD>
 struct Ring {
-    static constexpr int kTokens = HD == 64 ? 32 : 16, kStages = HD == 96 ? 4 : 3;       // of a stage; 12 KB in all
+    static constexpr int kTokens = HD == 64 ? 64 : 32, kStages = HD == 96 ? 3 : 2, kBlocks = 3;       // tokens of a stage, stages, blocks on an SM
     static constexpr uint32_t kHalf = kTokens * HD, kStage = 2 * kHalf;                 // keys, then values
     static constexpr uint32_t kBytes = kStages * kStage;
 };
@@ -164,7 +167,7 @@ struct Granule {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attention_kernel(const PagedArgs a) {
     using R = Ring<HD>;
     constexpr int KK = HD / 16, MT = HD / 16, NS = R::kStages, NG = R::kTokens / 16;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -177,6 +180,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
     const uint8_t *ring = smem + warp * R::kBytes;
     const uint32_t ring_at = smem_u32(ring), bar_at = smem_u32(&bars[warp][0]);
     const WaitCtl ctl{&abort_flag, a.wait};
+    // (asked for before anything that waits: the first of a chain of loads)
+    const int first_len = lane < a.B ? length_of(a, lane) : 0;
     if (threadIdx.x == 0) abort_flag = launch_aborted(a.wait);
     if (lane < NS) mbar_init(bar_at + 8 * lane, 1);
     fence_mbar_init();
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
     if (abort_flag) return;
     uint32_t issued = 0, used = 0;      // stages, counted through all of the run
     const int per_seq = a.n_kv * a.col_tiles, P = 1 << a.log_page, rows = a.group * a.n_new;
-    const Deal deal(units_between(a, 0, a.B) * per_seq, a.workers);
+    const Deal deal((warp_sum(units_of(first_len)) + (a.B > 32 ? units_between(a, 32, a.B) : 0)) * per_seq, a.workers);
     if (worker >= deal.workers) return;
     long long u = deal.first(worker);
     const long long u_end = deal.first(worker + 1), u_first = u;
@@ -194,7 +199,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
     int b = 0;
     long long base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-        long long n = b0 + lane < a.B ? units_of(length_of(a, b0 + lane)) * per_seq : 0, sum = n;
+        const long long n = units_of(b0 == 0 ? first_len : b0 + lane < a.B ? length_of(a, b0 + lane) : 0) * per_seq;
+        long long sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long x = __shfl_up_sync(0xffffffffu, sum, o);
@@ -254,47 +260,36 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
         };
         pages(page_base, id, ks, vs);
         float o[MT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        // Copies of the stage of tokens from `tok` on.  The warp has read what was there (it meets before each call).
+        // Copies of the stage of tokens from `tok` on.  The warp has read what was there (it meets before each call).  Lane 2 i copies the keys and
+        // lane 2 i + 1 the values of the stage's i-th page (or of the stage, where a page holds more); lane i writes down the scales of its i-th 16.
         auto load = [&](int tok) {
             const uint32_t st = issued++ % NS, dst = ring_at + st * R::kStage, bar = bar_at + 8 * st;
-            const int n = min(R::kTokens, (tok1 - tok + 15) & ~15), step = min(P, n);       // whole 16s: rows of a page exist, used or not
-            int pid[NG], at_lane[NG] = {};
-            uint32_t bytes = 0;
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                pid[i] = -1;
-                if (i * 16 < n) {
-                    int pi = ((tok + i * 16) >> a.log_page) - page_base;
-                    if (pi >= 32) {
-                        id = id2; ks = ks2; vs = vs2;       // (never between the 16s of a stage: pages of 16 come in fours)
-                        page_base += 32;
-                        pi -= 32;
-                        pages(page_base + 32, id2, ks2, vs2);
-                    }
-                    at_lane[i] = pi;
-                    pid[i] = __shfl_sync(0xffffffffu, id, pi);
-                    if (pid[i] >= 0) bytes += 2 * 16 * HD;
-                }
+            const int n = min(R::kTokens, (tok1 - tok + 15) & ~15), step = min(P, R::kTokens), page = tok >> a.log_page;      // (rows of a page exist, used or not)
+            if (page - page_base >= 32) {        // (pages come in whole stages)
+                id = id2; ks = ks2; vs = vs2;
+                page_base += 32;
+                pages(page_base + 32, id2, ks2, vs2);
             }
+            const int from = (lane >> 1) * step, at_copy = (from >> a.log_page) + page - page_base, at_scale = ((tok + lane * 16) >> a.log_page) - page_base;
+            const int pid = __shfl_sync(0xffffffffu, id, at_copy & 31), gid = __shfl_sync(0xffffffffu, id, at_scale & 31);
+            const float k = __shfl_sync(0xffffffffu, ks, at_scale & 31), v = __shfl_sync(0xffffffffu, vs, at_scale & 31);
+            const bool copies = from < n && pid >= 0;
+            const uint32_t size = copies ? (uint32_t)min(step, n - from) * HD : 0;
+            const uint32_t bytes = __reduce_add_sync(0xffffffffu, size);
             if (lane == 0) {
                 if (bytes) mbar_arrive_expect_tx(bar, bytes);
                 else mbar_arrive(bar);
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    // (a page of 32 or more holds the stage: one copy of each kind)
-                    if (i * 16 >= n || pid[i] < 0 || (i > 0 && step > 16)) continue;
-                    const long long at = (long long)pid[i] * a.page_stride + ((long long)head * P + ((tok + i * 16) & (P - 1))) * HD;
-                    const uint32_t size = (step > 16 ? n : 16) * HD;
-                    bulk_load(dst + i * 16 * HD, a.k + at, size, bar);
-                    bulk_load(dst + R::kHalf + i * 16 * HD, a.v + at, size, bar);
-                }
+            }
+            __syncwarp();
+            if (copies) {
+                const long long at = (long long)pid * a.page_stride + ((long long)head * P + ((tok + from) & (P - 1))) * HD;
+                bulk_load(dst + (lane & 1) * R::kHalf + from * HD, (lane & 1 ? a.v : a.k) + at, size, bar);
             }
             // (after the copies: they do not wait for the scales)
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const float k = __shfl_sync(0xffffffffu, ks, at_lane[i]), v = __shfl_sync(0xffffffffu, vs, at_lane[i]);
+            if (lane < NG) {
                 const int e = min(max((int)(__float_as_uint(v) >> 23 & 255) - 127, -kMaxExp), kMaxExp);
-                if (lane == 0) granules[warp][st][i] = Granule{pid[i] < 0 ? NAN : k, (float)e, v * __uint_as_float((uint32_t)(127 - e) << 23), 0.f};
+                granules[warp][st][lane] = lane * 16 < n && gid >= 0 ? Granule{k, (float)e, v * __uint_as_float((uint32_t)(127 - e) << 23), 0.f}
+                                                                     : Granule{NAN, 0.f, 1.f, 0.f};
             }
         };
         for (int i = 0; i < NS; ++i)
@@ -325,32 +320,45 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
             fac[0] = a.c * __shfl_sync(0xffffffffu, down, 8 * t);
             fac[1] = a.c * __shfl_sync(0xffffffffu, down, 8 * t + 4);
         }
-        auto compute = [&](int tok, const uint8_t *keys, const Granule st) {
-            const bool none = st.ks != st.ks;
-            const int left = none ? 0 : tok1 - tok;       // tokens of the 16 that are there; what lies behind them may be anything
-            float s[4] = {};
-            {
+        // 32 tokens: two chains of products, one look at the maximum.
+        auto compute = [&](int tok, const uint8_t *keys, const Granule *gr) {
+            const Granule st[2] = {gr[0], gr[1]};
+            float s[2][4] = {};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
                 uint32_t k0[HD / 16], k1[HD / 16];
-                load_words<HD / 16>(keys + g * HD + t * (HD / 4), k0);
-                load_words<HD / 16>(keys + (g + 8) * HD + t * (HD / 4), k1);
+                load_words<HD / 16>(keys + (16 * x + g) * HD + t * (HD / 4), k0);
+                load_words<HD / 16>(keys + (16 * x + g + 8) * HD + t * (HD / 4), k1);
 #pragma unroll
-                for (int i = 0; i < KK; ++i) mma16(s, half_pair(k0[i]), half_pair(k1[i]), half_pair_hi(k0[i]), half_pair_hi(k1[i]), qf[i][0], qf[i][1]);
+                for (int i = 0; i < KK; ++i) mma16(s[x], half_pair(k0[i]), half_pair(k1[i]), half_pair_hi(k0[i]), half_pair_hi(k1[i]), qf[i][0], qf[i][1]);
             }
-            uint32_t v[4][HD / 32];
+            uint32_t v[2][4][HD / 32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_words<HD / 32>(keys + R::kHalf + (2 * t + (i & 1) + 8 * (i >> 1)) * HD + g * (HD / 8), v[i]);
-            const float f0 = fac[0] * st.ks, f1 = fac[1] * st.ks;
-            s[0] = fmaf(s[0], f0, st.ve); s[1] = fmaf(s[1], f1, st.ve); s[2] = fmaf(s[2], f0, st.ve); s[3] = fmaf(s[3], f1, st.ve);
-            if (tok + 16 > min(all, tok1) || none) {
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (none || tok + g + 8 * (i >> 1) >= min(see[i & 1], tok1)) s[i] = -INFINITY;
-                    if (2 * t + (i & 1) + 8 * (i >> 1) >= left)
+                for (int i = 0; i < 4; ++i) load_words<HD / 32>(keys + R::kHalf + (16 * x + 2 * t + (i & 1) + 8 * (i >> 1)) * HD + g * (HD / 8), v[x][i]);
 #pragma unroll
-                        for (int w = 0; w < HD / 32; ++w) v[i][w] = 0;
+            for (int x = 0; x < 2; ++x) {
+                const float f0 = fac[0] * st[x].ks, f1 = fac[1] * st[x].ks;
+                s[x][0] = fmaf(s[x][0], f0, st[x].ve); s[x][1] = fmaf(s[x][1], f1, st[x].ve);
+                s[x][2] = fmaf(s[x][2], f0, st[x].ve); s[x][3] = fmaf(s[x][3], f1, st[x].ve);
+            }
+            if (tok + 32 > min(all, tok1) || st[0].ks != st[0].ks || st[1].ks != st[1].ks) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    // tokens of the 16 that are there (of no page: none); what lies behind them may be anything
+                    const bool none = st[x].ks != st[x].ks;
+                    const int from = tok + 16 * x, left = none ? 0 : tok1 - from;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (none || from + g + 8 * (i >> 1) >= min(see[i & 1], tok1)) s[x][i] = -INFINITY;
+                        if (2 * t + (i & 1) + 8 * (i >> 1) >= left)
+#pragma unroll
+                            for (int w = 0; w < HD / 32; ++w) v[x][i][w] = 0;
+                    }
                 }
             }
-            const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+            const float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
             if (__any_sync(0xffffffffu, x0 - m[0] > kLazyMax || x1 - m[1] > kLazyMax)) {
                 float n0 = x0, n1 = x1;
 #pragma unroll
@@ -368,27 +376,33 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
                 for (int i = 0; i < MT; ++i) { o[i][0] *= f0; o[i][1] *= f1; o[i][2] *= f0; o[i][3] *= f1; }
             }
             const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-            s[0] = ex2(s[0] - m0); s[1] = ex2(s[1] - m1); s[2] = ex2(s[2] - m0); s[3] = ex2(s[3] - m1);
-            const float weigh = __uint_as_float((uint32_t)(127 - (int)st.ve) << 23);
-            l[0] = fmaf(s[0] + s[2], weigh, l[0]);
-            l[1] = fmaf(s[1] + s[3], weigh, l[1]);
-            const uint32_t p0 = transpose8x8(pack_half(s[0], s[1])), p1 = transpose8x8(pack_half(s[2], s[3]));
-            const bool plain = st.vr == 1.f;
+            uint32_t p[2][2];
 #pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140), y = __byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140);
-                    if (plain) {
-                        mma16(o[2 * w + h], half_pair(x), half_pair_hi(x), half_pair(y), half_pair_hi(y), p0, p1);
-                    } else {
-                        float d[4] = {};
-                        mma16(d, half_pair(x), half_pair_hi(x), half_pair(y), half_pair_hi(y), p0, p1);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[2 * w + h][i] = fmaf(d[i], st.vr, o[2 * w + h][i]);
-                    }
-                }
+            for (int x = 0; x < 2; ++x) {
+                s[x][0] = ex2(s[x][0] - m0); s[x][1] = ex2(s[x][1] - m1); s[x][2] = ex2(s[x][2] - m0); s[x][3] = ex2(s[x][3] - m1);
+                const float weigh = __uint_as_float((uint32_t)(127 - (int)st[x].ve) << 23);
+                l[0] = fmaf(s[x][0] + s[x][2], weigh, l[0]);
+                l[1] = fmaf(s[x][1] + s[x][3], weigh, l[1]);
+                p[x][0] = transpose8x8(pack_half(s[x][0], s[x][1]));
+                p[x][1] = transpose8x8(pack_half(s[x][2], s[x][3]));
             }
+            const bool plain = st[0].vr == 1.f && st[1].vr == 1.f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int w = 0; w < HD / 32; ++w)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t y = __byte_perm(v[x][0][w], v[x][1][w], h ? 0x7362 : 0x5140), z = __byte_perm(v[x][2][w], v[x][3][w], h ? 0x7362 : 0x5140);
+                        if (plain) {
+                            mma16(o[2 * w + h], half_pair(y), half_pair_hi(y), half_pair(z), half_pair_hi(z), p[x][0], p[x][1]);
+                        } else {
+                            float d[4] = {};
+                            mma16(d, half_pair(y), half_pair_hi(y), half_pair(z), half_pair_hi(z), p[x][0], p[x][1]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[2 * w + h][i] = fmaf(d[i], st[x].vr, o[2 * w + h][i]);
+                        }
+                    }
         };
         for (int tok = tok0; tok < tok1; tok += R::kTokens, ++used) {
             const uint32_t st = used % NS;
@@ -398,8 +412,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) paged_attention_ker
                 return;
             }
 #pragma unroll
-            for (int i = 0; i < NG; ++i)
-                if (tok + 16 * i < tok1) compute(tok + 16 * i, ring + st * R::kStage + i * 16 * HD, granules[warp][st][i]);
+            for (int i = 0; i < NG; i += 2)
+                if (tok + 16 * i < tok1) compute(tok + 16 * i, ring + st * R::kStage + i * 16 * HD, &granules[warp][st][i]);
             __syncwarp();
             if (tok + NS * R::kTokens < tok1) load(tok + NS * R::kTokens);
         }
@@ -520,14 +534,14 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
     if (a.lse && threadIdx.x == 0) a.lse[((long long)b * a.n_new + n) * a.n_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-int workers_for(int num_sms) { return num_sms * kBlocksPerSm * kWarps; }
+int workers_for(int num_sms, int hd) { return num_sms * kWarps * (hd == 64 ? Ring<64>::kBlocks : hd == 96 ? Ring<96>::kBlocks : Ring<128>::kBlocks); }
 
 }  // namespace
 
 int col_tiles_of(const flashmhf_paged_attention_params &p) { return (p.n_q / p.pages.n_kv * p.n_new + kCols - 1) / kCols; }
 
 size_t paged_attention_workspace_bytes(const flashmhf_paged_attention_params &p) {
-    return (size_t)workers_for(num_sms()) * 2 * kCols * (p.pages.head_dim + 2) * sizeof(float) +
+    return (size_t)workers_for(num_sms(), p.pages.head_dim) * 2 * kCols * (p.pages.head_dim + 2) * sizeof(float) +
            (size_t)p.seq.B * p.pages.n_kv * col_tiles_of(p) * sizeof(int4);
 }
 
@@ -544,7 +558,7 @@ int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &c
     a.log_page = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
     a.group = p.n_q / g.n_kv;
     a.col_tiles = col_tiles_of(p);
-    a.workers = workers_for(ctl.num_sms);
+    a.workers = workers_for(ctl.num_sms, g.head_dim);
     a.part = static_cast<float *>(p.workspace);
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)a.workers * 2 * kCols * g.head_dim);
     a.shared_by = reinterpret_cast<int4 *>(a.ml + (size_t)a.workers * 2 * kCols);
