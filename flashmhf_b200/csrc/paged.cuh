@@ -25,9 +25,13 @@ __device__ __forceinline__ float scale_for(uint32_t amax_bits) {
     return __uint_as_float((uint32_t)(n + 127) << 23);
 }
 
-// Two codes of (a, b) * inv, rounded to nearest even; NaN and infinities become NaN (x - x is 0 for every finite x).
+// 1 / 2^n of a scale 2^n (n <= 120, the most that scale_for gives).
+__device__ __forceinline__ float inverse_scale(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
+
+// Two codes of (a, b) * inv, rounded to nearest even.  Not ALL_FINITE: NaN and infinities become NaN (x - x is 0 for every finite x).
+template <bool ALL_FINITE>
 __device__ __forceinline__ uint32_t to_codes2(float a, float b, float inv) {
-    const float2 v = make_float2(fmaf(a, inv, a - a), fmaf(b, inv, b - b));
+    const float2 v = ALL_FINITE ? make_float2(a * inv, b * inv) : make_float2(fmaf(a, inv, a - a), fmaf(b, inv, b - b));
     return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
 }
 

@@ -3,6 +3,8 @@
 // One launch does all of it: its blocks are split between "pages" (one page, key/value head and K or V each: the scale of a page
 // depends on all of its new rows, so one block sees them all; of single tokens sixteen to a block) and "queries".  A page's new rows stay in registers between the
 // maximum and the rounding, so everything is read once and written once: bound by HBM for prompts, by latency for single tokens.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "tc_common.cuh"
 
@@ -24,10 +26,9 @@ struct AppendArgs {
     unsigned page_blocks;    // blocks of the first kind
 };
 
-// PAIRS neighbouring bf16 at an address that is a multiple of 2 * PAIRS bytes (PAIRS in {4, 6, 8}), as fp32, and back.
+// PAIRS neighbouring bf16 at an address that is a multiple of 2 * PAIRS bytes (PAIRS in {4, 6, 8}), as they are and as fp32, and back.
 template <int PAIRS>
-__device__ __forceinline__ void load_bf16(const __nv_bfloat16 *p, float (&f)[PAIRS]) {
-    uint32_t w[PAIRS / 2];
+__device__ __forceinline__ void load_raw(const __nv_bfloat16 *p, uint32_t (&w)[PAIRS / 2]) {
     if constexpr (PAIRS == 8) {
         const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
         w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
@@ -38,11 +39,20 @@ __device__ __forceinline__ void load_bf16(const __nv_bfloat16 *p, float (&f)[PAI
 #pragma unroll
         for (int i = 0; i < PAIRS / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
     }
+}
+template <int PAIRS>
+__device__ __forceinline__ void to_float(const uint32_t (&w)[PAIRS / 2], float (&f)[PAIRS]) {
 #pragma unroll
     for (int i = 0; i < PAIRS / 2; ++i) {
         f[2 * i] = __uint_as_float(w[i] << 16);
         f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+}
+template <int PAIRS>
+__device__ __forceinline__ void load_bf16(const __nv_bfloat16 *p, float (&f)[PAIRS]) {
+    uint32_t w[PAIRS / 2];
+    load_raw<PAIRS>(p, w);
+    to_float<PAIRS>(w, f);
 }
 template <int PAIRS>
 __device__ __forceinline__ void store_bf16(__nv_bfloat16 *p, const float (&f)[PAIRS]) {
@@ -65,11 +75,11 @@ __device__ __forceinline__ void load_f32(const float *p, float (&f)[PAIRS]) {
     }
 }
 // PAIRS codes of f * inv at an address that is a multiple of PAIRS bytes (of 2 for PAIRS = 6).
-template <int PAIRS>
+template <int PAIRS, bool ALL_FINITE>
 __device__ __forceinline__ void store_codes(uint8_t *p, const float (&f)[PAIRS], float inv) {
     uint32_t h[PAIRS / 2];
 #pragma unroll
-    for (int i = 0; i < PAIRS / 2; ++i) h[i] = to_codes2(f[2 * i], f[2 * i + 1], inv);
+    for (int i = 0; i < PAIRS / 2; ++i) h[i] = to_codes2<ALL_FINITE>(f[2 * i], f[2 * i + 1], inv);
     if constexpr (PAIRS == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     else if constexpr (PAIRS == 4) *reinterpret_cast<uint32_t *>(p) = h[0] | h[1] << 16;
     else
@@ -88,12 +98,20 @@ __device__ __forceinline__ void rotate(float (&x1)[PAIRS], float (&x2)[PAIRS], c
         x2[i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
     }
 }
+// The largest magnitude so far, by its bits: of every value (above kInf: there is a NaN), and of the finite ones.
+constexpr uint32_t kInf = 0x7f800000u;
+template <int PAIRS>
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const float (&f)[PAIRS]) {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+    return m;
+}
 template <int PAIRS>
 __device__ __forceinline__ uint32_t max_finite(uint32_t m, const float (&f)[PAIRS]) {
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
         const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
-        m = max(m, b < 0x7f800000u ? b : 0u);
+        m = max(m, b < kInf ? b : 0u);
     }
     return m;
 }
@@ -118,84 +136,110 @@ __device__ __forceinline__ Piece piece_of(const AppendArgs &a, int b) {
 
 // Blocks of the first kind, by their number: slot, head, K or V.  Sequence b owns the slots from cu[b] / P + 2 b on, at least as many as
 // the pages that its new tokens can touch (floor((n - 1) / P) + 2 at most); which sequence a slot belongs to is a binary search.
-template <int HD>
-__device__ void append_page(const AppendArgs &a, int P, uint32_t *red) {
-    constexpr int PAIRS = HD / 16, kMaxPasses = 4;       // eight threads a row; at most 128 rows by 256 threads, or 16 by 128
-    const int kv2 = 2 * a.n_kv;
+// Eight threads a row, PASSES rows a thread, kept in registers between the maximum and the codes.  Up to 32 values are kept turned and in
+// fp32; more are kept as the bf16 that were read and turned twice, which lets a second block onto an SM (eight prompts of 4096, 128 wide:
+// 180 -> 162 us).  The rows are asked for before the page that they go to is known.
+template <int HD, int PASSES>
+__device__ void append_page(const AppendArgs &a, int log2_p, uint32_t *red) {
+    constexpr int PAIRS = HD / 16;
+    constexpr bool KEEP = PASSES * PAIRS <= 16;
+    const int P = 1 << log2_p, kv2 = 2 * a.n_kv;
     const int slot = (int)(blockIdx.x / (unsigned)kv2), hk = (int)(blockIdx.x % (unsigned)kv2), head = hk >> 1, which = hk & 1;
     int b = 0, hi = a.B - 1;
     while (b < hi) {
         const int mid = (b + hi + 1) >> 1;
-        if (__ldg(a.cu + mid) / P + 2 * mid <= slot) b = mid;
+        if ((__ldg(a.cu + mid) >> log2_p) + 2 * mid <= slot) b = mid;
         else hi = mid - 1;
     }
-    const int j = slot - (__ldg(a.cu + b) / P + 2 * b);
+    const int j = slot - ((__ldg(a.cu + b) >> log2_p) + 2 * b);
     const Piece pc = piece_of(a, b);
     if (pc.last <= pc.first || j < 0) return;
     // (64 bits: a length near 2^31 is the caller's mistake, not a wrap-around)
-    const long long end = (long long)pc.before + (pc.last - pc.first), page_no = (long long)(pc.before / P) + j, start = page_no * P;
+    const long long end = (long long)pc.before + (pc.last - pc.first), page_no = (long long)(pc.before >> log2_p) + j, start = page_no << log2_p;
     if (start >= end) return;
-    if (page_no >= a.max_pages) {
-        if (threadIdx.x == 0) note_index(a.status, kPagedAppendPage);
-        return;
+    const int had = (int)max(0ll, pc.before - start);                       // rows that are there already
+    const int row_end = (int)min(min((long long)P, end - start), max(0ll, a.max_pos - start));
+    const int rows_per_pass = blockDim.x >> 3, sub = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+    const long long tok0 = pc.first + (start - pc.before);                  // the token of the page's row 0
+    const __nv_bfloat16 *x = a.x[which] + head * a.x_head[which] + sub * PAIRS;
+    uint32_t w1[PASSES][PAIRS / 2], w2[PASSES][PAIRS / 2];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int row = row0 + i * rows_per_pass;
+        if (row >= had && row < row_end) {
+            const __nv_bfloat16 *src = x + (tok0 + row) * a.x_tok[which];
+            load_raw<PAIRS>(src, w1[i]);
+            load_raw<PAIRS>(src + HD / 2, w2[i]);
+        }
     }
-    const int page = __ldg(a.table + b * a.table_stride + page_no);
+    const int page = page_no < a.max_pages ? __ldg(a.table + b * a.table_stride + page_no) : -1;
     if (page < 0 || page >= a.num_pages) {
         if (threadIdx.x == 0) note_index(a.status, kPagedAppendPage);
         return;
     }
-    const int had = (int)max(0ll, pc.before - start);                       // rows that are there already
-    const int row_end = (int)min((long long)P, end - start);
-    const int rows_per_pass = blockDim.x >> 3, sub = threadIdx.x & 7, row0 = threadIdx.x >> 3;
-    float y1[kMaxPasses][PAIRS], y2[kMaxPasses][PAIRS];
-    uint32_t amax = 0;
-    bool bad = false;
-    const __nv_bfloat16 *x = a.x[which];
-#pragma unroll
-    for (int i = 0; i < kMaxPasses; ++i) {
-        const int row = row0 + i * rows_per_pass;
-        const long long pos = start + row;
-        const bool in = row >= had && row < row_end;
-        if (in && pos < a.max_pos) {
-            const long long t = pc.first + (pos - pc.before);
-            const __nv_bfloat16 *src = x + t * a.x_tok[which] + head * a.x_head[which] + sub * PAIRS;
-            load_bf16<PAIRS>(src, y1[i]);
-            load_bf16<PAIRS>(src + HD / 2, y2[i]);
-            if (which == 0) {
-                float c[PAIRS], s[PAIRS];
-                load_f32<PAIRS>(a.cos_t + pos * (HD / 2) + sub * PAIRS, c);
-                load_f32<PAIRS>(a.sin_t + pos * (HD / 2) + sub * PAIRS, s);
-                rotate<PAIRS>(y1[i], y2[i], c, s);
-                if (a.k_out) {
-                    __nv_bfloat16 *dst = a.k_out + (t * a.n_kv + head) * HD + sub * PAIRS;
-                    store_bf16<PAIRS>(dst, y1[i]);
-                    store_bf16<PAIRS>(dst + HD / 2, y2[i]);
-                }
-            }
-            amax = max_finite<PAIRS>(max_finite<PAIRS>(amax, y1[i]), y2[i]);
-        } else if (in) {
-            bad = true;
-        }
-    }
-    if (bad) note_index(a.status, kPagedAppendPosition);
-    amax = __reduce_max_sync(0xffffffffu, amax);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-    __syncthreads();
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) amax = max(amax, red[i]);
+    if (threadIdx.x == 0 && min((long long)P, end - start) > row_end) note_index(a.status, kPagedAppendPosition);
     float *sp = a.scale[which] + (long long)page * a.n_kv + head;
-    const float old = *sp, need = scale_for(amax), now = had > 0 ? fmaxf(old, need) : need;
-    const float inv = 1.f / now;                 // exact: a power of two
-    uint8_t *dst = a.pages[which] + page * a.page_stride + (long long)head * P * HD;
-    __syncthreads();                             // every thread has read the scale
-    if (threadIdx.x == 0) *sp = now;
+    const float old = had > 0 ? *sp : 0.f;
+    float y1[KEEP ? PASSES : 1][PAIRS], y2[KEEP ? PASSES : 1][PAIRS];
+    auto values = [&](int i, float (&v1)[PAIRS], float (&v2)[PAIRS]) {
+        to_float<PAIRS>(w1[i], v1);
+        to_float<PAIRS>(w2[i], v2);
+        if (which == 0) {
+            const long long pos = start + row0 + i * rows_per_pass;
+            float c[PAIRS], s[PAIRS];
+            load_f32<PAIRS>(a.cos_t + pos * (HD / 2) + sub * PAIRS, c);
+            load_f32<PAIRS>(a.sin_t + pos * (HD / 2) + sub * PAIRS, s);
+            rotate<PAIRS>(v1, v2, c, s);
+        }
+    };
+    uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < kMaxPasses; ++i) {
-        const int row = row0 + i * rows_per_pass;
-        if (row >= had && row < row_end && start + row < a.max_pos) {
-            store_codes<PAIRS>(dst + row * HD + sub * PAIRS, y1[i], inv);
-            store_codes<PAIRS>(dst + row * HD + HD / 2 + sub * PAIRS, y2[i], inv);
+    for (int i = 0; i < PASSES; ++i) {
+        const int row = row0 + i * rows_per_pass, k = KEEP ? i : 0;
+        if (row >= had && row < row_end) {
+            values(i, y1[k], y2[k]);
+            amax = max_bits<PAIRS>(max_bits<PAIRS>(amax, y1[k]), y2[k]);
+            if (which == 0 && a.k_out) {
+                __nv_bfloat16 *dst = a.k_out + ((tok0 + row) * a.n_kv + head) * HD + sub * PAIRS;
+                store_bf16<PAIRS>(dst, y1[k]);
+                store_bf16<PAIRS>(dst + HD / 2, y2[k]);
+            }
         }
     }
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    const bool all_finite = amax < kInf;             // of this warp
+    if (!all_finite) {
+        amax = 0;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int row = row0 + i * rows_per_pass, k = KEEP ? i : 0;
+            if (row >= had && row < row_end) {
+                if constexpr (!KEEP) values(i, y1[k], y2[k]);
+                amax = max_finite<PAIRS>(max_finite<PAIRS>(amax, y1[k]), y2[k]);
+            }
+        }
+        amax = __reduce_max_sync(0xffffffffu, amax);
+    }
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    __syncthreads();                                 // (every thread has read the scale, too)
+    amax = __reduce_max_sync(0xffffffffu, red[threadIdx.x & (blockDim.x / 32 - 1)]);
+    const float need = scale_for(amax), now = had > 0 ? fmaxf(old, need) : need;
+    const float inv = inverse_scale(now);
+    uint8_t *dst = a.pages[which] + page * a.page_stride + (long long)head * P * HD;
+    if (threadIdx.x == 0 && row_end > had) *sp = now;
+    auto store = [&](auto finite) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int row = row0 + i * rows_per_pass, k = KEEP ? i : 0;
+            if (row >= had && row < row_end) {
+                if constexpr (!KEEP) values(i, y1[k], y2[k]);
+                store_codes<PAIRS, decltype(finite)::value>(dst + row * HD + sub * PAIRS, y1[k], inv);
+                store_codes<PAIRS, decltype(finite)::value>(dst + row * HD + HD / 2 + sub * PAIRS, y2[k], inv);
+            }
+        }
+    };
+    if (all_finite) store(std::true_type{});
+    else store(std::false_type{});
     if (had > 0 && now != old) {
         const float ratio = old * inv;
         for (int i = threadIdx.x; i < had * (HD / 16); i += blockDim.x) {
@@ -208,7 +252,7 @@ __device__ void append_page(const AppendArgs &a, int P, uint32_t *red) {
 
 // One token a sequence: eight threads a (sequence, head, K or V).  The page's other rows are touched only where its scale grows.
 template <int HD>
-__device__ void append_token(const AppendArgs &a, int P) {
+__device__ void append_token(const AppendArgs &a, int log2_p) {
     constexpr int PAIRS = HD / 16;
     const long long it = (long long)blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3);
     const int sub = threadIdx.x & 7, which = (int)(it & 1), head = (int)((it >> 1) % a.n_kv);
@@ -222,7 +266,7 @@ __device__ void append_token(const AppendArgs &a, int P) {
     load_bf16<PAIRS>(src + HD / 2, y2);
     const int pos = __ldg(a.lengths + b);
     if (pos < 0) return;
-    const int page_no = pos / P, row = pos % P;
+    const int P = 1 << log2_p, page_no = pos >> log2_p, row = pos & (P - 1);
     const int page = page_no < a.max_pages ? __ldg(a.table + b * a.table_stride + page_no) : -1;
     if (page < 0 || page >= a.num_pages || pos >= a.max_pos) {
         note_index(a.status, page < 0 || page >= a.num_pages ? kPagedAppendPage : kPagedAppendPosition);
@@ -244,12 +288,12 @@ __device__ void append_token(const AppendArgs &a, int P) {
     uint32_t amax = max_finite<PAIRS>(max_finite<PAIRS>(0, y1), y2);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(group, amax, o));
-    const float need = scale_for(amax), now = row > 0 ? fmaxf(old, need) : need, inv = 1.f / now;
+    const float need = scale_for(amax), now = row > 0 ? fmaxf(old, need) : need, inv = inverse_scale(now);
     uint8_t *dst = a.pages[which] + page * a.page_stride + (long long)head * P * HD;
     __syncwarp(group);                           // all eight have read the scale
     if (sub == 0 && now != old) *sp = now;
-    store_codes<PAIRS>(dst + row * HD + sub * PAIRS, y1, inv);
-    store_codes<PAIRS>(dst + row * HD + HD / 2 + sub * PAIRS, y2, inv);
+    store_codes<PAIRS, false>(dst + row * HD + sub * PAIRS, y1, inv);
+    store_codes<PAIRS, false>(dst + row * HD + HD / 2 + sub * PAIRS, y2, inv);
     if (row > 0 && now != old) {
         const float ratio = old * inv;
 #pragma unroll 4
@@ -309,12 +353,13 @@ __device__ void append_queries(const AppendArgs &a) {
     }
 }
 
-template <int HD>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int P) {
+// PASSES: rows of a page that a thread takes; 0: one token a sequence.
+template <int HD, int PASSES>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int log2_p) {
     __shared__ uint32_t red[8];
     if (blockIdx.x >= a.page_blocks) append_queries<HD>(a);
-    else if (a.cu) append_page<HD>(a, P, red);
-    else append_token<HD>(a, P);
+    else if constexpr (PASSES > 0) append_page<HD, PASSES>(a, log2_p, red);
+    else append_token<HD>(a, log2_p);
 }
 
 }  // namespace
@@ -344,8 +389,11 @@ int paged_append(const flashmhf_paged_append_params &p, const DeviceCtl &ctl, cu
     const long long blocks = page_blocks + ((long long)p.tokens * groups + per_block - 1) / per_block;
     if (blocks > 0x7fffffffll) return FLASHMHF_ERR_BAD_SHAPE;
     a.page_blocks = (unsigned)page_blocks;
-    auto kernel = g.head_dim == 64 ? paged_append_kernel<64> : g.head_dim == 96 ? paged_append_kernel<96> : paged_append_kernel<128>;
-    const cudaError_t e = launch_kernel(false, kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a, P);
+    auto choose = [&](auto k0, auto k1, auto k2, auto k4) { return !a.cu ? k0 : P == 128 ? k4 : P == 64 ? k2 : k1; };
+    auto kernel = g.head_dim == 64   ? choose(paged_append_kernel<64, 0>, paged_append_kernel<64, 1>, paged_append_kernel<64, 2>, paged_append_kernel<64, 4>)
+                  : g.head_dim == 96 ? choose(paged_append_kernel<96, 0>, paged_append_kernel<96, 1>, paged_append_kernel<96, 2>, paged_append_kernel<96, 4>)
+                                     : choose(paged_append_kernel<128, 0>, paged_append_kernel<128, 1>, paged_append_kernel<128, 2>, paged_append_kernel<128, 4>);
+    const cudaError_t e = launch_kernel(false, kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a, __builtin_ctz((unsigned)P));
     if (e != cudaSuccess) {
         set_cuda_error(e, "paged append launch");
         return FLASHMHF_ERR_CUDA;
