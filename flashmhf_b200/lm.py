@@ -506,6 +506,8 @@ class DecoderLM(nn.Module):
         into one pass whatever their lengths.  Returns the logits [len(prompts), vocab] for the token after each, in that order of places."""
         places = sorted(prompts)
         for b in places:
+            if not 0 <= b < len(cache.held):
+                raise ValueError(f"place {b} is not one of the cache's {len(cache.held)}")
             if cache.held[b] >= 0:
                 raise ValueError(f"place {b} of the cache holds a sequence: release it first")
             if prompts[b].dim() != 1 or prompts[b].numel() == 0:
@@ -518,14 +520,18 @@ class DecoderLM(nn.Module):
             starts.append(starts[-1] + n)
         cu = torch.tensor(starts, dtype=torch.int32, device=device)
         at = torch.tensor(places, device=device)
-        cache.lengths[at] = 0
-        for b in places:
-            cache.held[b] = 0
         ids = torch.cat([prompts[b].to(device) for b in places])
-        h = self._paged(ids[None], cache, None, cu)[0]
+        cache.lengths[at] = 0
+        try:
+            h = self._paged(ids[None], cache, None, cu)[0]
+        except BaseException:
+            for b in places:
+                cache.release(b)
+            raise
         new = torch.tensor(counts, dtype=torch.int32, device=device)
         cache.lengths[at] = new[at]
-        cache.advance(counts)
+        for b in places:
+            cache.held[b] = counts[b]
         return self.lm_head(h[cu[1:][at].long() - 1])
 
     @torch.no_grad()

@@ -52,3 +52,7 @@ def test_prefill_refuses_places_in_use_and_empty_prompts():
         m.prefill_paged({1: ids[None]}, c)
     with pytest.raises((TypeError, ValueError)):   # CPU tensors: the operators have no CPU path
         m.prefill_paged({1: ids}, c)
+    assert c.held == [3, -1] and c.owned[1] == [] and len(c.free) == 3 and c.lengths.tolist() == [-1, -1]     # as before the call
+    for b in (2, -1):
+        with pytest.raises(ValueError, match="place"):
+            m.prefill_paged({b: ids}, c)
