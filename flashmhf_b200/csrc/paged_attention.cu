@@ -568,8 +568,8 @@ int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &c
     a.wait = wait_args(&ctl);
     auto kernel = g.head_dim == 64 ? paged_attention_kernel<64> : g.head_dim == 96 ? paged_attention_kernel<96> : paged_attention_kernel<128>;
     // An item has workers / items parts where its sequence is as long as the others, and up to all of them where it is the only long one.
-    // With few items there are few rows as well, and a block of 16 warps for each costs nothing: two of 65537 tokens, 296 parts an item,
-    // XXX us by four warps, XXX by sixteen; 64 of 8192, five parts, XXX and XXX.
+    // With few items there are few rows as well, and a block of 16 warps for each costs nothing: two of 65537 tokens, over 200 parts
+    // an item, 53 us by four warps, 39 by sixteen; 64 of 8192, about four parts, 183 and 212.
     const bool wide = (long long)a.B * g.n_kv * a.col_tiles * 16 <= a.workers;
     auto combine = g.head_dim == 64   ? (wide ? paged_combine_kernel<64, 16> : paged_combine_kernel<64, 4>)
                    : g.head_dim == 96 ? (wide ? paged_combine_kernel<96, 16> : paged_combine_kernel<96, 4>)

@@ -3,6 +3,7 @@
     python opbench.py --sweep      # operator forward+backward over a grid of shapes, next to a dense SwiGLU and the eager path on the GPU
     python opbench.py --lm         # forward tokens/s of the 128M and 1.3B LMs, training step of the 370M LM
     python opbench.py --decode     # decode-shaped forward calls (a few tokens, weights streamed from HBM)
+    python opbench.py --serve      # prompts of uneven lengths into a paged 8-bit cache, then one token a step from it
 
 Everything is timed with CUDA events after warm-up; inputs are seeded synthetic tensors (Q ~ N(0,1),
 weights ~ N(0, 0.02), routing weights = normalised sigmoid of N(0,1) logits, dO ~ N(0,1)).
@@ -238,21 +239,76 @@ def decode_runs(args):
         del outs, gr, gc, Ws
 
 
+def serve_runs(args):
+    """Prompts of uneven lengths are packed, eight to a pass, into a PagedKVCache; then every sequence gets one token a step (the arg-max of the
+    logits) from a captured step.  The decode step reads the weights and what the cache holds once."""
+    from flashmhf_b200 import lm
+    dev = torch.device("cuda")
+    print("| model | sequences, tokens each | prefill ms | prefill tokens/s | step ms | tokens/s | weights + cache GB a step | GB/s |")
+    print("|---|---|---|---|---|---|---|---|")
+    for name, cfg, B, longest in (("370M", lm.LMConfig.lm_370m(), 8, 1024), ("1.3B", lm.LMConfig.lm_1p3b(), 64, 4096)):
+        model = lm.DecoderLM(cfg).init_weights(seed=0).to(dev).to(torch.bfloat16)
+        g = torch.Generator().manual_seed(0)
+        counts = torch.randint(longest // 2, longest + 1, (B,), generator=g).tolist()
+        prompts = [torch.randint(0, cfg.vocab_size, (n,), generator=g).to(dev) for n in counts]
+        steps = 64
+        cache = lm.PagedKVCache(cfg, B, sum(-(-(n + 3 * steps) // 64) for n in counts), max_len=longest + 3 * steps, device=dev)
+
+        def prefill():
+            for b in range(B):
+                cache.release(b)
+            return torch.cat([model.prefill_paged({b: prompts[b] for b in range(i, min(i + 8, B))}, cache) for i in range(0, B, 8)])
+        pre_ms = _time(prefill, target_s=0.5)
+        ids = prefill().argmax(-1)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ids.copy_(model.decode_step_paged(ids, cache).argmax(-1))
+        torch.cuda.current_stream().wait_stream(side)
+        step = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(step):
+            ids.copy_(model.decode_step_paged(ids, cache).argmax(-1))
+
+        def run():
+            cache.reserve(1)
+            step.replay()
+            cache.advance(1)
+        for _ in range(3):
+            run()
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        torch.cuda.synchronize()
+        ev[0].record()
+        for _ in range(steps):
+            run()
+        ev[1].record()
+        torch.cuda.synchronize()
+        ms = ev[0].elapsed_time(ev[1]) / steps
+        tables = 0 if cfg.tie_word_embeddings else model.model.embed_tokens.weight.numel()      # (a step reads a few of its rows)
+        nbytes = 2 * (lm.param_count(model) - tables) + cache.nbytes()
+        print(f"| {name} | {B}, {min(counts)} to {max(counts)} | {pre_ms:.2f} | {sum(counts) / (pre_ms * 1e-3):.0f} | {ms:.3f} | {B / (ms * 1e-3):.0f} | "
+              f"{nbytes / 1e9:.2f} | {nbytes / (ms * 1e-3) / 1e9:.0f} |", flush=True)
+        del step, model, cache
+        torch.cuda.empty_cache()
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--sweep", action="store_true")
     ap.add_argument("--lm", action="store_true")
     ap.add_argument("--decode", action="store_true")
+    ap.add_argument("--serve", action="store_true")
     ap.add_argument("--quick", action="store_true", help="a quarter of the sweep grid")
     args = ap.parse_args()
-    if not (args.sweep or args.lm or args.decode):
-        ap.error("choose --sweep, --lm and/or --decode")
+    if not (args.sweep or args.lm or args.decode or args.serve):
+        ap.error("choose --sweep, --lm, --decode and/or --serve")
     if args.sweep:
         sweep(args)
     if args.lm:
         lm_runs(args)
     if args.decode:
         decode_runs(args)
+    if args.serve:
+        serve_runs(args)
 
 
 if __name__ == "__main__":
