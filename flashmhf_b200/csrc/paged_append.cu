@@ -2,7 +2,10 @@
 //
 // One launch does all of it: its blocks are split between "pages" (one page, key/value head and K or V each: the scale of a page
 // depends on all of its new rows, so one block sees them all; of single tokens sixteen to a block) and "queries".  A page's new rows stay in registers between the
-// maximum and the rounding, so everything is read once and written once: bound by HBM for prompts, by latency for single tokens.
+// maximum and the rounding, so everything is read once and written once.  Bound: single tokens by latency (one launch: 128 sequences take as long
+// as one); prompts by HBM with heads of 128 (eight of 4096 tokens, 807 MB: 144 us = 5.6 TB/s), and by instructions and the chain of loads before
+// the first row with heads of 64, whose pages are a block's work of 8 KB (74 MB in pieces: 24 us = 3.1 TB/s; blocks that went through
+// several heads, asking for the next one's rows ahead, took 31 and 246 us: too many registers).
 #include <type_traits>
 
 #include "paged.cuh"
@@ -137,8 +140,8 @@ __device__ __forceinline__ Piece piece_of(const AppendArgs &a, int b) {
 // Blocks of the first kind, by their number: slot, head, K or V.  Sequence b owns the slots from cu[b] / P + 2 b on, at least as many as
 // the pages that its new tokens can touch (floor((n - 1) / P) + 2 at most); which sequence a slot belongs to is a binary search.
 // Eight threads a row, PASSES rows a thread, kept in registers between the maximum and the codes.  Up to 32 values are kept turned and in
-// fp32; more are kept as the bf16 that were read and turned twice, which lets a second block onto an SM (eight prompts of 4096, 128 wide:
-// 180 -> 162 us).  The rows are asked for before the page that they go to is known.
+// fp32; more are kept as the bf16 that were read and turned twice, at half the registers (eight prompts of 4096, heads of 128, pages of
+// 128: 180 -> 162 us).  The rows are asked for before the page that they go to is known.
 template <int HD, int PASSES>
 __device__ void append_page(const AppendArgs &a, int log2_p, uint32_t *red) {
     constexpr int PAIRS = HD / 16;
@@ -353,9 +356,12 @@ __device__ void append_queries(const AppendArgs &a) {
     }
 }
 
-// PASSES: rows of a page that a thread takes; 0: one token a sequence.
+// PASSES: rows of a page that a thread takes; 0: one token a sequence.  Blocks that an SM is to hold, against the compiler's choice: eight prompts
+// of 4096 tokens, heads of 128 in pages of 128 (three blocks, not two) 153 -> 144 us, of 64 (four, not three) 145 -> 139.
 template <int HD, int PASSES>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int log2_p) {
+constexpr int kMinBlocks = HD == 64 ? 5 : HD == 128 && PASSES == 4 ? 3 : 4;
+template <int HD, int PASSES>
+__global__ void __launch_bounds__(256, kMinBlocks<HD, PASSES>) paged_append_kernel(const AppendArgs a, int log2_p) {
     __shared__ uint32_t red[8];
     if (blockIdx.x >= a.page_blocks) append_queries<HD>(a);
     else if constexpr (PASSES > 0) append_page<HD, PASSES>(a, log2_p, red);
