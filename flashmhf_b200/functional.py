@@ -82,6 +82,6 @@ def flash_mhf(Q, K, U, V, R, head_scaling=1.0, up_scaling=1.0, final_scaling=1.0
 
 def check_device_status():
     """Synchronise and raise FlashMHFError if a kernel of this library gave up on a bounded wait (its outputs are then
-    unwritten).  The entry points only enqueue work, so this is the place a host loop learns of it: call it where the
+    unwritten) or a serving kernel left out what a page number, length or position out of range asked for.  The entry points only enqueue work, so this is the place a host loop learns of it: call it where the
     loop synchronises anyway (after the loss is read back, at the end of a step)."""
     _lib.device_status()
