@@ -470,7 +470,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
     const int n = r / a.group, h = head * a.group + r % a.group, col = r % kCols;
     const bool empty = length_of(a, b) == 0;
     griddep_wait();        // launched early, behind the kernel whose parts it adds
-    const int4 by = empty ? make_int4(0, 0, 0, 0) : a.shared_by[((long long)b * a.n_kv + head) * a.col_tiles + r / kCols];
+    int4 by = empty ? make_int4(0, 0, 0, 0) : a.shared_by[((long long)b * a.n_kv + head) * a.col_tiles + r / kCols];
+    // (a warp that gave up on a wait has written nothing, neither here nor of its parts: what stands there may be anything)
+    by = make_int4(min(max(by.x, 0), a.workers - 1), min(max(by.y, 0), a.workers - 1), by.z & 1, 0);
     if (!empty && by.x == by.y) return;
     float m = -INFINITY, l = 0.f;
     if (!empty) {
