@@ -325,7 +325,95 @@ def test_prompt_attention_sequences_do_not_touch_each_other():
         assert torch.equal(o.cpu()[keep], clean.cpu()[keep])
 
 
+@pytest.mark.parametrize("hd,scale,size", [(64, -0.5, 1.0), (128, 0.0, 1.0), (64, 2.0, 4.0), (96, 0.1, 60.0), (128, -0.7, 8.0)])
+def test_prompt_attention_scales_and_scores_that_grow(hd, scale, size):
+    """Scores up to some thousands, growing along the keys, so that the maximum of a row moves by far many times; scales of zero and below it.
+    A score is hd / 16 products in fp32, each off by 2^-22 of the sum of its magnitudes at most, and its argument is rounded three times more:
+    weights are off by that many times the largest score besides their own rounding."""
+    import flashmhf_b200 as fm
+    n, heads, kv = [700, 129], 4, 2
+    q, k, v = _packed(sum(n), heads, hd, 1, size), _packed(sum(n), kv, hd, 2), _packed(sum(n), kv, hd, 3)
+    k = (k * torch.linspace(0.2, 2, sum(n))[:, None, None]).bfloat16()
+    want, want_lse, room = _prompt_reference(q, k, v, n, n, scale, True)
+    most = float((q.double().abs().amax(0) * 1.0).norm(dim=-1).max() * k.double().norm(dim=-1).max()) * abs(scale)
+    off = most * (hd / 16 * 2.0 ** -22 + 3 * 2.0 ** -24)
+    o, lse = fm.prompt_attention(q.cuda(), k.cuda(), v.cuda(), ref.ints(_starts(n)), scale=scale, return_lse=True)
+    _close(o, want, room * (1 + 2 * off * 2.0 ** 8), lse, want_lse)
+
+
 # ------------------------------------------------------------------------------------------------ all of them
+def test_two_streams_at_once_and_a_replayed_graph():
+    """The three calls in a row, on two streams at once, then captured and replayed with other lengths, pages and prompts: as one by one."""
+    import flashmhf_b200 as fm
+    hd, kv, heads, P = 64, 2, 4, 16
+    cos, sin = ref.tables(600, hd)
+    x = _packed(300, heads + 2 * kv, hd, 7).cuda()
+    q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+
+    def state(counts, seed):
+        rows, n = ref.page_tables([c + 1 for c in counts], P, seed=seed, spare=40 - sum(-(-(c + 1) // P) for c in counts))
+        rows = [r + [-1] * (30 - len(r)) for r in rows]
+        return _pool(n, kv, P, hd, seed), ref.ints(counts), ref.ints(rows), ref.ints(_starts(counts))
+
+    def run(pages, counts, rows, cu):
+        none = torch.zeros_like(counts)
+        qr, kr = fm.paged_append(pages, k, v, cos, sin, none, rows, q=q, cu_seqlens=cu, rotated_keys=True)
+        o = torch.zeros(300, heads, hd, dtype=torch.bfloat16, device="cuda")
+        fm.prompt_attention(qr, kr, v, cu, out=o)
+        q1, _ = fm.paged_append(pages, k[:3], v[:3], cos, sin, counts, rows, q=q[:3])
+        return o, fm.paged_attention(q1, pages, counts + 1, rows)
+
+    cases = [([100, 3, 190], 1), ([1, 250, 40], 2)]
+    want = [run(*state(*c)) for c in cases]
+    streams, states = [torch.cuda.Stream() for _ in cases], [state(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = run(*states[i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    held = state(*cases[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*held)
+    for i in (1, 0, 1):
+        for t, new in zip(held[1:], states[i][1:]):
+            t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want[i], out))
+
+
+def test_pages_behind_two_and_four_gigabytes():
+    """Offsets of pages that pass 31 and 32 bits, in bytes and in elements."""
+    import flashmhf_b200 as fm
+    hd, kv, P = 128, 8, 128
+    n = 2 ** 32 // (kv * P * hd) + 40
+    pages = fm.KVPages.empty(n, kv, P, hd)
+    rows = [[n - 1, 3, n // 2 + 1], [n - 7, n // 2 - 1, 5]]
+    counts, heads = [300, 270], 8
+    x = _packed(sum(counts), heads + 2 * kv, hd, 3).cuda()
+    q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    cos, sin = ref.tables(400, hd)
+    fm.paged_append(pages, k, v, cos, sin, ref.ints([0, 0]), ref.ints(rows), cu_seqlens=ref.ints(_starts(counts)))
+    small = fm.KVPages(*(t[torch.tensor(sum(rows, []), device="cuda")].clone() if t.dim() == 2 else
+                         t.view(torch.uint8)[torch.tensor(sum(rows, []), device="cuda")].clone().view(t.dtype) for t in pages))
+    near = [[0, 1, 2], [3, 4, 5]]
+    again = fm.KVPages.empty(6, kv, P, hd)
+    fm.paged_append(again, k, v, cos, sin, ref.ints([0, 0]), ref.ints(near), cu_seqlens=ref.ints(_starts(counts)))
+    for b, (a, m) in enumerate(zip(near, counts)):
+        for j, page in enumerate(a):
+            rows_here = min(P, m - j * P)
+            for one, two in zip(small[:2], again[:2]):
+                assert torch.equal(one[page, :, :rows_here].view(torch.uint8), two[page, :, :rows_here].view(torch.uint8))
+            assert all(torch.equal(one[page], two[page]) for one, two in zip(small[2:], again[2:]))
+    last = q[[counts[0] - 1, sum(counts) - 1]]
+    assert torch.equal(fm.paged_attention(last, pages, ref.ints(counts), ref.ints(rows)), fm.paged_attention(last, again, ref.ints(counts), ref.ints(near)))
+
+
 def test_nothing_to_do():
     import flashmhf_b200 as fm
     pages = fm.KVPages.empty(2, 2, 16, 64)
