@@ -475,9 +475,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 const float x = fmaxf(max3(top[0], top[1], top[2]), top[3]);
                 if (!__all_sync(0xffffffffu, heard) && !warp_wait(msg_in, ((step - 1) >> 1) & 1, ctl, W + 16)) { ok = false; break; }
                 const float was = j > 0 ? refs[(par ^ 1) * kRows] : -INFINITY;
-                // (the first finite maximum of a row is always taken: -inf is exceeded by more than anything)
-                const bool any = __any_sync(0xffffffffu, (x - was) * c > kLazy);
-                const float ref = any ? fmaxf(was, x) : was;
+                // (the first finite maximum of a row is always taken: -inf is exceeded by more than anything.  A row decides for itself: rows of
+                // the next sequence, or of none, must not show in this one's last bits)
+                const bool over = (x - was) * c > kLazy, any = __any_sync(0xffffffffu, over);
+                const float ref = over ? x : was;
                 refs[par * kRows] = ref;
                 warp_arrive(msg_out);
                 if (any && j > 0) {

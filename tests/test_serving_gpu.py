@@ -325,6 +325,23 @@ def test_prompt_attention_sequences_do_not_touch_each_other():
         assert torch.equal(o.cpu()[keep], clean.cpu()[keep])
 
 
+def test_prompt_attention_gives_the_same_bits_among_any_neighbours():
+    """Rows next to a sequence's last tile, of another sequence or of none, do not show in it, however large they are."""
+    import flashmhf_b200 as fm
+    n, heads, hd = [130, 190, 5], 2, 64
+    a, b = 130, 320
+    q, k, v = (_packed(sum(n), heads, hd, i) for i in (1, 2, 3))
+    alone = fm.prompt_attention(q[a:b].cuda(), k[a:b].cuda(), v[a:b].cuda(), ref.ints([0, 190]))
+    for size in (1.0, 1e3, 1e30):
+        x = [t.clone() for t in (q, k, v)]
+        for t in x:
+            t[:a] *= size
+            t[b:] *= size
+        for cu in (_starts(n), [a, b]):
+            o = fm.prompt_attention(*(t.cuda() for t in x), ref.ints(cu))
+            assert torch.equal(o[a:b], alone)
+
+
 @pytest.mark.parametrize("hd,scale,size", [(64, -0.5, 1.0), (128, 0.0, 1.0), (64, 2.0, 4.0), (96, 0.1, 60.0), (128, -0.7, 8.0)])
 def test_prompt_attention_scales_and_scores_that_grow(hd, scale, size):
     """Scores up to some thousands, growing along the keys, so that the maximum of a row moves by far many times; scales of zero and below it.
