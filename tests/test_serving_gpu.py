@@ -257,6 +257,9 @@ PROMPT = [  # rows, keys (None: the same), kv, heads, hd, causal
     ([40, 200], [333, 2], 3, 3, 96, False),
     ([1, 1, 1], [300, 1, 128], 2, 4, 64, True),
     ([1300], None, 1, 2, 64, True),
+    ([7, 0, 30, 1] * 100, None, 1, 7, 64, True),        # several heads a block
+    ([200] * 50 + [3, 600], None, 2, 10, 128, True),
+    ([90, 150] * 25, [40, 300] * 25, 13, 13, 96, False),
 ]
 
 
