@@ -23,8 +23,8 @@
 // takes over one that has not started (clusterlaunchcontrol) while it works on its own.
 //
 // Warp roles: 0-3 and 4-7 softmax of the even and the odd steps (warp % 4 = TMEM lane quarter = 32 rows), 8 work items and TMA, 9 issues S, 10 O
-// += P V and clears the rows of V behind the end of a sequence (a weight of 0 does not undo a NaN of the next one), 12-15 write out an item's rows
-// while the others are at the next.
+// += P V and clears the rows of V behind the end of a sequence (a weight of 0 does not undo a NaN of the next one), 11 TMA of the values (heads above
+// 64), 12-15 write out an item's rows while the others are at the next.
 #include <atomic>
 
 #include "paged.cuh"
@@ -47,6 +47,10 @@ template <int HD>
 struct PromptCfg {
     static constexpr int kChunks = (HD + 63) / 64, kStages = HD == 64 ? 4 : 2;
     static constexpr uint32_t kChunk = kRows * 128;             // 64 columns of a tile
+    // With two stages the loader's thread waits for values while keys could go on: a warp of their own loads them (16 / 4 heads of 128:
+    // 64 prompts of 300 rows 117 -> 99 us, 37 of 512 97 -> 89, 18 of 1024 121 -> 115, one of 8192 235 -> 236).  With four it seldom waits, and such a warp
+    // only lets it take work further ahead than is well for the balance (heads of 64: 37 of 512 73 -> 76, 592 of 16 125 -> 140).
+    static constexpr bool kValueWarp = kStages == 2;
     static_assert(kRows == kKeys, "tiles of Q, K and V are of one size");
     static constexpr uint32_t kTile = kChunks * kChunk;
     static constexpr uint32_t kOffQ = 0, kOffK = 2 * kTile, kOffV = kOffK + kStages * kTile;
@@ -191,7 +195,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     auto bar = [&](int i) { return sBar + 8u * i; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtl ctl{abort_flag, args.wait};
-    constexpr int W = kKernelPrompt * 100, kLoad = kSoftmaxWarps, kIssue = kLoad + 1, kOut = kLoad + 4;
+    constexpr int W = kKernelPrompt * 100, kLoad = kSoftmaxWarps, kIssue = kLoad + 1, kValues = kLoad + 3, kOut = kLoad + 4;
 
     if (threadIdx.x == 0) {
         *abort_flag = launch_aborted(args.wait);
@@ -209,7 +213,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         }
         for (int i = 0; i < kItems; ++i) {
             mbar_init(bar(PB_ITEMFULL + i), 1);
-            mbar_init(bar(PB_ITEMEMPTY + i), kSoftmaxWarps + 6);      // softmax, both issuers, output
+            mbar_init(bar(PB_ITEMEMPTY + i), kSoftmaxWarps + 6 + L::kValueWarp);      // softmax, both issuers, output
         }
         for (int i = 0; i < 8; ++i) mbar_init(bar(PB_MSG + i), 1);
         mbar_init(bar(PB_NEXT), 1);
@@ -238,6 +242,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         read_item(seq, w);
         warp_arrive(bar(PB_ITEMEMPTY + seq % kItems));
         return w.head >= 0;
+    };
+
+    // Tile j of an item's values, tile g of all; one thread.
+    auto load_values = [&](uint32_t g, const PromptItem &w, int head, int j) -> bool {
+        const uint32_t st = g % NS;
+        if (!thread_wait(bar(PB_VEMPTY + st), (g / NS & 1) ^ 1, ctl, W + 5)) return false;
+        const uint32_t full = bar(((j + 1) * kKeys > w.lk ? PB_VRAW : PB_VFULL) + st);
+        mbar_arrive_expect_tx(full, L::kTile);
+        for (int c = 0; c < L::kChunks; ++c) tma_load_3d(sV + st * L::kTile + c * L::kChunk, &tmV, full, c * 64, head, w.k0 + j * kKeys);
+        return true;
     };
 
     if (*abort_flag) {
@@ -330,7 +344,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                                 tma_load_3d(sQ + qb * L::kTile + c * L::kChunk, &tmQ, bar(PB_QFULL + qb), c * 64, w.head, w.q0);
                         }
                         const int kh = w.head / args.group;
-                        // keys of tile j, then values of tile j - 1, which are needed that much later: keys never wait for a stage of values
+                        // keys of tile j, then (without a warp for them) values of tile j - 1, which are needed that much later: keys never wait for a
+                        // stage of values
                         for (int j = 0; ok && j <= n && n > 0; ++j) {
                             if (j < n) {
                                 const uint32_t st = (g + j) % NS;
@@ -339,13 +354,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                                 for (int c = 0; c < L::kChunks; ++c)
                                     tma_load_3d(sK + st * L::kTile + c * L::kChunk, &tmK, bar(PB_KFULL + st), c * 64, kh, w.k0 + j * kKeys);
                             }
-                            if (j > 0) {
-                                const uint32_t st = (g + j - 1) % NS;
-                                if (!thread_wait(bar(PB_VEMPTY + st), ((g + j - 1) / NS & 1) ^ 1, ctl, W + 5)) { ok = false; break; }
-                                const uint32_t full = bar((j * kKeys > w.lk ? PB_VRAW : PB_VFULL) + st);
-                                mbar_arrive_expect_tx(full, L::kTile);
-                                for (int c = 0; c < L::kChunks; ++c) tma_load_3d(sV + st * L::kTile + c * L::kChunk, &tmV, full, c * 64, kh, w.k0 + (j - 1) * kKeys);
-                            }
+                            if (!L::kValueWarp && j > 0) ok = load_values(g + j - 1, w, kh, j - 1);
                         }
                         g += n;
                     }
@@ -361,6 +370,21 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         : "memory");
                     fence_async_smem();          // the answer has been read before the next one is written there
                     index = got ? (int)next : -1;
+                }
+            }
+        } else if (L::kValueWarp && warp == kValues) {
+            // -------------------------------------------------------------- TMA of the values
+            if (lane == 0) {
+                PromptItem w;
+                uint32_t g = 0;           // tiles so far
+                bool ok = true;
+                for (unsigned seq = 0; ok; ++seq) {
+                    if (!thread_wait(bar(PB_ITEMFULL + seq % kItems), seq / kItems & 1, ctl, W + 22)) break;
+                    read_item(seq, w);
+                    mbar_arrive(bar(PB_ITEMEMPTY + seq % kItems));
+                    if (w.head < 0) break;
+                    const int kh = w.head / args.group;
+                    for (int j = 0; ok && j < w.n; ++j, ++g) ok = load_values(g, w, kh, j);
                 }
             }
         } else if (warp == kIssue) {
