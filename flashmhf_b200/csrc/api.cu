@@ -423,6 +423,11 @@ int flashmhf_lm_add_rmsnorm_backward(const void *sum, const void *w, int32_t w_d
     return rc;
 }
 
+// A softmax scale that is finite, and so is its product with log2(e), which the kernels multiply by.
+static bool scale_ok(float scale) {
+    const float c = scale * 1.4426950408889634f;
+    return c - c == 0.f;
+}
 // bf16 rows of the serving calls: innermost dimension contiguous, everything else in steps of 16 bytes.
 static int check_rows(const void *p, const int64_t *stride, int n) {
     if (!p) return FLASHMHF_ERR_NULL;
@@ -471,7 +476,7 @@ static int check_paged_attention(const flashmhf_paged_attention_params *p) {
     if (!p) return FLASHMHF_ERR_NULL;
     int rc = check_pages(p->pages, p->seq);
     if (rc) return rc;
-    if (p->n_q < 1 || p->n_q > 65535 || p->n_q % p->pages.n_kv != 0 || p->n_new < 1 || p->n_new > 16 || !(p->scale - p->scale == 0.f))
+    if (p->n_q < 1 || p->n_q > 65535 || p->n_q % p->pages.n_kv != 0 || p->n_new < 1 || p->n_new > 16 || !scale_ok(p->scale))
         return FLASHMHF_ERR_BAD_SHAPE;
     if ((rc = check_rows(p->q, p->q_stride, 3)) != 0 || (rc = check_rows(p->o, p->o_stride, 3)) != 0) return rc;
     return reinterpret_cast<uintptr_t>(p->lse) & 3u ? FLASHMHF_ERR_MISALIGNED : FLASHMHF_OK;
@@ -499,7 +504,7 @@ int flashmhf_prompt_attention(const flashmhf_prompt_attention_params *p, void *s
     if (!p) return FLASHMHF_ERR_NULL;
     if (p->head_dim != 64 && p->head_dim != 96 && p->head_dim != 128) return FLASHMHF_ERR_BAD_SHAPE;
     if (p->B < 1 || p->tokens_q < 1 || p->tokens_k < 0 || p->n_kv < 1 || p->n_q < 1 || p->n_q > 65535 || p->n_q % p->n_kv != 0 ||
-        !(p->scale - p->scale == 0.f))
+        !scale_ok(p->scale))
         return FLASHMHF_ERR_BAD_SHAPE;
     int rc = FLASHMHF_OK;
     if ((rc = check_rows(p->q, p->q_stride, 2)) != 0 || (rc = check_rows(p->k, p->k_stride, 2)) != 0 || (rc = check_rows(p->v, p->v_stride, 2)) != 0 ||

@@ -87,8 +87,9 @@ struct PromptArgs {
     float *lse;
     const int32_t *cu_q, *cu_k;
     int B, tokens_q, tokens_k, n_q, group, causal, heads, n_blocks;
-    float c;             // |scale| log2(e), at least a tiny number (masked scores are -inf, and 0 times that is not a number)
-    int negate;          // scale < 0
+    // scale log2(e) is c * before, c > 0: scores are multiplied by `before` as they come, and by c in the exponent, behind the mask.  `before` is the sign,
+    // but where |scale| log2(e) is below 2^-60 it is all of it and c is 1: a c of 0 would make no number of a masked score's -inf.
+    float c, before;
     WaitArgs wait;
 };
 
@@ -491,9 +492,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 warp_arrive(bar(PB_SFREE + par));
                 // Asked here, needed behind the maximum: has the step before said what it was taken with?
                 const bool heard = step == 0 || mbar_test(msg_in, ((step - 1) >> 1) & 1);
-                if (args.negate)
+                if (args.before != 1.f)
 #pragma unroll
-                    for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
+                    for (int i = 0; i < kKeys; ++i) s[i] *= args.before;
                 if ((j + 1) * kKeys > all) {
                     const int left = see - j * kKeys;
 #pragma unroll
@@ -638,9 +639,10 @@ int prompt_attention(const flashmhf_prompt_attention_params &p, const DeviceCtl 
     const long long blocks = slots * ((p.n_q + a.heads - 1) / a.heads);
     if (blocks > 0x3fffffffll) return FLASHMHF_ERR_BAD_SHAPE;
     a.n_blocks = (int)blocks;
-    a.negate = p.scale < 0.f;
-    const float c = (p.scale < 0.f ? -p.scale : p.scale) * 1.4426950408889634f;
-    a.c = c > 1e-30f ? c : 1e-30f;
+    const float c = p.scale * 1.4426950408889634f, size = c < 0.f ? -c : c;
+    const bool tiny = size < 0x1p-60f;
+    a.c = tiny ? 1.f : size;
+    a.before = tiny ? c : c < 0.f ? -1.f : 1.f;
     a.wait = wait_args(&ctl);
     switch (p.head_dim) {
         case 64: return launch_prompt<64>(p, a, ctl.device, st, n_launch);

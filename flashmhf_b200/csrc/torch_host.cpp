@@ -837,7 +837,7 @@ Tensor given_or_new(const std::optional<Tensor> &out, const Tensor &like) {
 }
 float softmax_scale(const std::optional<double> &scale, int64_t hd) {
     const double s = scale ? *scale : 1.0 / std::sqrt((double)hd);
-    if (!std::isfinite(s)) throw py::value_error("scale must be finite");
+    if (!std::isfinite((float)s * 1.4426950408889634f)) throw py::value_error("scale must be finite, and its product with log2(e) in fp32 too");
     return (float)s;
 }
 

@@ -327,7 +327,7 @@ typedef struct flashmhf_paged_attention_params {
     void *workspace;
     size_t workspace_bytes;
     int32_t n_q, n_new;               /* n_new in 1 .. 16 */
-    float scale;
+    float scale;                      /* finite, and so is scale * log2(e) */
 } flashmhf_paged_attention_params;
 size_t flashmhf_paged_attention_workspace_bytes(const flashmhf_paged_attention_params *p);
 int flashmhf_paged_attention(const flashmhf_paged_attention_params *p, void *stream);
@@ -343,7 +343,7 @@ typedef struct flashmhf_prompt_attention_params {
     float *lse;
     const int32_t *cu_q, *cu_k;       /* [B+1] */
     int32_t B, tokens_q, tokens_k, n_q, n_kv, head_dim, causal;
-    float scale;
+    float scale;                      /* finite, and so is scale * log2(e) */
 } flashmhf_prompt_attention_params;
 int flashmhf_prompt_attention(const flashmhf_prompt_attention_params *p, void *stream);
 
