@@ -23,7 +23,7 @@
 // takes over one that has not started (clusterlaunchcontrol) while it works on its own.
 //
 // Warp roles: 0-3 and 4-7 softmax of the even and the odd steps (warp % 4 = TMEM lane quarter = 32 rows), 8 work items and TMA, 9 issues S, 10 O
-// += P V and clears the rows of V behind the end of a sequence (a weight of 0 does not undo a NaN of the next one), 11 TMA of the values (heads above
+// += P V and clears the rows of V behind the last key that a row of the item sees (a weight of 0 does not undo a NaN), 11 TMA of the values (heads above
 // 64), 12-15 write out an item's rows while the others are at the next.
 #include <atomic>
 
@@ -75,7 +75,7 @@ static_assert(kOffCtl + 8 <= kControl, "control area");
 
 struct PromptItem {
     int q0, lq;          // first row of the item in the packed rows; rows of the sequence from there on
-    int k0, lk;          // first key and keys of the sequence
+    int k0, lk;          // first key of the sequence, and keys from there on that the item's last row sees
     int see;             // keys that the item's first row sees, before clamping: row r sees min(lk, see + r) (causal) or lk
     int n;               // tiles of keys
     int head;            // -1: no more items
@@ -114,10 +114,11 @@ __device__ __forceinline__ bool prompt_item(const PromptArgs &a, int index, Prom
     w.q0 = q0 + r0;
     w.lq = lq - r0;
     w.k0 = k0;
-    w.lk = lk;
     w.see = a.causal ? r0 + 1 + lk - lq : lk;
-    const int most = a.causal ? min(lk, max(0, w.see + min(kRows, w.lq) - 1)) : lk;      // keys that the last row sees
-    w.n = (most + kKeys - 1) / kKeys;
+    // Keys behind those are nobody's here, like those behind the sequence: their values are cleared (a weight of 0 does not undo a NaN).  So a value
+    // reaches rows of its own tile only, 127 before its own at most, wherever the tiles of keys begin.
+    w.lk = a.causal ? min(lk, max(0, w.see + min(kRows, w.lq) - 1)) : lk;
+    w.n = (w.lk + kKeys - 1) / kKeys;
     return true;
 }
 

@@ -34,3 +34,21 @@ def test_prompt_attention_scales_near_the_ends_of_their_range(hd, scale, size):
     off = most * (hd / 16 * 2.0 ** -22 + 6 * 2.0 ** -24)
     o, lse = fm.prompt_attention(q.cuda(), k.cuda(), v.cuda(), ref.ints(_starts(n)), scale=scale, return_lse=True)
     _close(o, want, room * (1 + 2 * off * 2.0 ** 8), lse, want_lse)
+
+
+@pytest.mark.parametrize("lq,lk", [(300, 300), (300, 301), (300, 427), (300, 299), (130, 700)])
+@pytest.mark.parametrize("bad", [0, 100, 255, 256, 290])
+def test_prompt_attention_values_that_are_no_numbers_reach_127_rows_at_most(lq, lk, bad):
+    """Whatever the difference between rows and keys: row r sees key c where c <= r + lk - lq, and a value at c that is not a number may reach
+    the 127 rows before its own, no other row that does not see it."""
+    import flashmhf_b200 as fm
+    q, k, v = _packed(lq + 9, 2, 64, 1), _packed(lk + 9, 2, 64, 2), _packed(lk + 9, 2, 64, 3)
+    cu_q, cu_k = ref.ints([0, lq, lq + 9]), ref.ints([0, lk, lk + 9])
+    clean = fm.prompt_attention(q.cuda(), k.cuda(), v.cuda(), cu_q, cu_k)
+    v[bad] = NAN
+    o = fm.prompt_attention(q.cuda(), k.cuda(), v.cuda(), cu_q, cu_k)
+    own = bad - (lk - lq)                      # the first row that sees it
+    untouched = torch.ones(lq + 9, dtype=torch.bool)
+    untouched[max(0, own - 127):lq] = False
+    assert torch.equal(o.cpu()[untouched], clean.cpu()[untouched])
+    assert bool(o.cpu()[max(0, own):lq].isnan().all())
