@@ -43,8 +43,12 @@ struct Ring {
 // largest P is 2^7, and set again when one exceeds 2^15: fp16 holds P to 11 bits down to 2^-21 of the largest product of weight and
 // scale, and in steps of 2^-31 of it below.  e is kept within +-45 (what a scale is beyond that multiplies the product instead), so that
 // the sum of the weights themselves, P 2^-e, loses nothing in fp32 to pages whose values are larger.
+// Where the scales of the pages that a run knows (32 to 64 ahead) are more than 2^8 apart, P of the smaller ones would lose its bits to the larger ones'
+// m, though other dimensions may hold nothing but theirs.  There the weights of 16 tokens have an m of their own, which puts their largest between 2^6 and
+// 2^7; what it differs from the run's multiplies their product in fp32, as the rest of a scale does that is not a power of two or beyond
+// 2^+-45.  Either way a weight is off by 2^-11 of itself, or by 2^-24 of the row's largest.
 constexpr float kTop = 7.f, kLazyMax = 15.f;
-constexpr int kMaxExp = 45;
+constexpr int kMaxExp = 45, kFar = 8;
 
 struct PagedArgs {
     const uint8_t *k, *v;
@@ -161,9 +165,11 @@ struct Deal {
     }
 };
 
-// What a stage's pages stand for, by its 16 tokens: key scale (NaN: no page), exponent of the value scale (clamped), the rest of that scale.
+// What a stage's pages stand for, by its 16 tokens: key scale (NaN: no page), exponent of the value scale (clamped), the rest of that scale;
+// `plain`: that is 1, and the run's scales are not far apart.
 struct Granule {
-    float ks, ve, vr, pad;
+    float ks, ve, vr;
+    int plain;
 };
 
 template <int HD>
@@ -173,6 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attentio
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) unsigned long long bars[kWarps][NS];
     __shared__ Granule granules[kWarps][NS][NG];
+    __shared__ int2 spans[kWarps];      // least and largest exponent of the values' scales, of the pages that a warp's run knows so far
     __shared__ int abort_flag;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int worker = blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -265,7 +272,8 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attentio
         auto load = [&](int tok) {
             const uint32_t st = issued++ % NS, dst = ring_at + st * R::kStage, bar = bar_at + 8 * st;
             const int n = min(R::kTokens, (tok1 - tok + 15) & ~15), step = min(P, R::kTokens), page = tok >> a.log_page;      // (rows of a page exist, used or not)
-            if (page - page_base >= 32) {        // (pages come in whole stages)
+            const bool more = page - page_base >= 32;
+            if (more) {        // (pages come in whole stages)
                 id = id2; ks = ks2; vs = vs2;
                 page_base += 32;
                 pages(page_base + 32, id2, ks2, vs2);
@@ -286,10 +294,17 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attentio
                 bulk_load(dst + (lane & 1) * R::kHalf + from * HD, (lane & 1 ? a.v : a.k) + at, size, bar);
             }
             // (after the copies: they do not wait for the scales)
+            auto exponent = [](float scale) { return min(max((int)(__float_as_uint(scale) >> 23 & 255) - 127, -kMaxExp), kMaxExp); };
+            if (more || tok == tok0) {
+                const int ev = exponent(vs), least = __reduce_min_sync(0xffffffffu, id >= 0 ? ev : kMaxExp), most = __reduce_max_sync(0xffffffffu, id >= 0 ? ev : -kMaxExp);
+                if (lane == 0) spans[warp] = more ? make_int2(min(spans[warp].x, least), max(spans[warp].y, most)) : make_int2(least, most);
+                __syncwarp();
+            }
             if (lane < NG) {
-                const int e = min(max((int)(__float_as_uint(v) >> 23 & 255) - 127, -kMaxExp), kMaxExp);
-                granules[warp][st][lane] = lane * 16 < n && gid >= 0 ? Granule{k, (float)e, v * __uint_as_float((uint32_t)(127 - e) << 23), 0.f}
-                                                                     : Granule{NAN, 0.f, 1.f, 0.f};
+                const int e = exponent(v);
+                const float vr = v * __uint_as_float((uint32_t)(127 - e) << 23);
+                granules[warp][st][lane] = lane * 16 < n && gid >= 0 ? Granule{k, (float)e, vr, vr == 1.f && spans[warp].y - spans[warp].x <= kFar}
+                                                                     : Granule{NAN, 0.f, 1.f, 1};
             }
         };
         for (int i = 0; i < NS; ++i)
@@ -376,17 +391,35 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attentio
                 for (int i = 0; i < MT; ++i) { o[i][0] *= f0; o[i][1] *= f1; o[i][2] *= f0; o[i][3] *= f1; }
             }
             const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+            const bool plain = st[0].plain & st[1].plain;
             uint32_t p[2][2];
+            float back[2][2];             // not plain: what the products of 16 tokens and their sums of weights are multiplied by
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                s[x][0] = ex2(s[x][0] - m0); s[x][1] = ex2(s[x][1] - m1); s[x][2] = ex2(s[x][2] - m0); s[x][3] = ex2(s[x][3] - m1);
-                const float weigh = __uint_as_float((uint32_t)(127 - (int)st[x].ve) << 23);
-                l[0] = fmaf(s[x][0] + s[x][2], weigh, l[0]);
-                l[1] = fmaf(s[x][1] + s[x][3], weigh, l[1]);
+                s[x][0] -= m0; s[x][1] -= m1; s[x][2] -= m0; s[x][3] -= m1;
+                float w0 = __uint_as_float((uint32_t)(127 - (int)st[x].ve) << 23), w1 = w0;
+                if (!plain) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = fmaxf(s[x][i], s[x][i + 2]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        // a whole number of powers of two; 16 tokens that weigh less than 2^-120 of the run's product may go
+                        const float up = fminf(fmaxf(floorf(kTop - top), -kLazyMax), 120.f);
+                        s[x][i] += up;
+                        s[x][i + 2] += up;
+                        back[x][i] = __uint_as_float((uint32_t)(127 - (int)up) << 23);
+                    }
+                    w0 *= back[x][0];
+                    w1 *= back[x][1];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[x][i] = ex2(s[x][i]);
+                l[0] = fmaf(s[x][0] + s[x][2], w0, l[0]);
+                l[1] = fmaf(s[x][1] + s[x][3], w1, l[1]);
                 p[x][0] = transpose8x8(pack_half(s[x][0], s[x][1]));
                 p[x][1] = transpose8x8(pack_half(s[x][2], s[x][3]));
             }
-            const bool plain = st[0].vr == 1.f && st[1].vr == 1.f;
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -400,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attentio
                             float d[4] = {};
                             mma16(d, half_pair(y), half_pair_hi(y), half_pair(z), half_pair_hi(z), p[x][0], p[x][1]);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) o[2 * w + h][i] = fmaf(d[i], st[x].vr, o[2 * w + h][i]);
+                            for (int i = 0; i < 4; ++i) o[2 * w + h][i] = fmaf(d[i], st[x].vr * back[x][i & 1], o[2 * w + h][i]);
                         }
                     }
         };

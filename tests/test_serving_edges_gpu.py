@@ -52,3 +52,45 @@ def test_prompt_attention_values_that_are_no_numbers_reach_127_rows_at_most(lq, 
     untouched[max(0, own - 127):lq] = False
     assert torch.equal(o.cpu()[untouched], clean.cpu()[untouched])
     assert bool(o.cpu()[max(0, own):lq].isnan().all())
+
+
+def _strict(got, want, room, heaviest, size):
+    """One bf16 rounding of the output; weights in fp16 (11 bits of themselves, and 2^-24 of the row's heaviest below that) times values of summed
+    size ``size``; and scores and sums in fp32 (2^-16 of the weights)."""
+    err = (got.double().cpu() - want).abs()
+    most = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -16) * room + 2.0 ** -24 * heaviest * size + 1e-30
+    assert bool((err <= most).all()), float((err / most).max())
+
+
+def _one_head(q, k, v, scale):
+    """q [rows, hd], k, v [n, hd] -> output, weighted sizes, heaviest weights, sizes; 64 bits, CPU."""
+    w = torch.softmax(q.double() @ k.T * scale, -1)
+    return w @ v, w @ v.abs(), w.amax(-1, keepdim=True), v.abs().sum(0)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("ratio", [6, 12, 26, 30, 50, 80])
+@pytest.mark.parametrize("order", [1, -1])
+def test_paged_attention_pages_of_very_different_scales(hd, ratio, order):
+    """Pages with large values in some dimensions and pages with small ones in the others, 2^ratio apart: each dimension has the accuracy of its
+    own values, whichever page comes first."""
+    import flashmhf_b200 as fm
+    P, n, G = 16, 150, 3
+    pages = fm.KVPages.empty(10, 1, P, hd)
+    g = torch.Generator().manual_seed(ratio)
+    kc = torch.randn(10, 1, P, hd, generator=g).mul(30).to(torch.float8_e4m3fn)
+    vc = torch.randn(10, 1, P, hd, generator=g).mul(60).clamp(-448, 448)
+    big = torch.zeros(10, dtype=torch.bool)
+    big[::order * 3 if order > 0 else 4] = True
+    if order < 0:
+        big = big.flip(0)
+    vc[big, ..., hd // 2:] = 0
+    vc[~big, ..., :hd // 2] = 0
+    vc = vc.to(torch.float8_e4m3fn)
+    scale = torch.where(big, 2.0 ** (ratio // 2), 2.0 ** (ratio // 2 - ratio))[:, None]
+    pages.k.copy_(kc), pages.v.copy_(vc), pages.v_scale.copy_(scale), pages.k_scale.fill_(2.0 ** -5)
+    K, V = ((c.double() * s).reshape(-1, hd)[:n] for c, s in ((kc, 2.0 ** -5), (vc, scale[:, :, None, None].double())))
+    for size in (0.0, 1.0):
+        q = (torch.randn(1, G, hd, generator=g) * size).bfloat16()
+        o = fm.paged_attention(q.cuda(), pages, ref.ints([n]), ref.ints([list(range(10))]))
+        _strict(o[0], *_one_head(q[0], K, V, hd ** -0.5))
