@@ -536,12 +536,15 @@ class DecoderLM(nn.Module):
 
     @torch.no_grad()
     def decode_step_paged(self, ids, cache):
-        """One token more for every sequence of a PagedKVCache: ids [batch] (of a place without a sequence: any).  Returns the logits [batch, vocab]
+        """One token more for every sequence of a PagedKVCache: ids [batch] (of a place without a sequence: any number).  Returns the logits [batch, vocab]
         for the token after it.  Captured into a CUDA graph only the device's part is recorded (see PagedKVCache)."""
+        if ids.shape != cache.lengths.shape:
+            raise ValueError(f"ids must be [{cache.lengths.shape[0]}], one for each place of the cache, got {list(ids.shape)}")
         host = not (ids.is_cuda and torch.cuda.is_current_stream_capturing())
         if host:
             cache.reserve(1)
         lengths = cache.lengths + (cache.lengths >= 0)
+        ids = ids.masked_fill(cache.lengths < 0, 0)      # (what stands in an empty place need not be a token: the embedding must not look it up)
         h = self._paged(ids[:, None], cache, lengths)
         cache.lengths.copy_(lengths)
         if host:

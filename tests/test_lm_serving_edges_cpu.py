@@ -1,0 +1,40 @@
+"""CPU: what callers of the LM's serving paths may do at the edges: empty places, places outside the batch, calls that fail half way."""
+import pytest
+import torch
+
+from flashmhf_b200 import lm, serving
+from tests.test_lm_serving_cpu import CFG, _begin
+
+
+def _model():
+    return lm.DecoderLM(CFG, ffn=lambda x, p, **k: x).init_weights(seed=0)
+
+
+@pytest.fixture
+def plain_operators(monkeypatch):
+    """Stand-ins on the CPU that keep shapes and nothing else."""
+    monkeypatch.setattr(serving, "paged_append", lambda pages, k, v, *a, q=None, cu_seqlens=None, rotated_keys=False: (q, k if rotated_keys else None))
+    monkeypatch.setattr(serving, "paged_attention", lambda q, *a: q)
+    monkeypatch.setattr(serving, "prompt_attention", lambda q, *a: q)
+
+
+@pytest.mark.parametrize("filler", [-1, -100, 50, 2**31])
+def test_ids_of_empty_places_may_be_anything(filler, plain_operators):
+    """They are looked up in no embedding; the other places' logits do not depend on them."""
+    m, out = _model(), []
+    for x in (filler, 0):
+        c = lm.PagedKVCache(CFG, 3, 6, page_size=16, device="cpu")
+        _begin(c, 1, 3)
+        c.lengths[1] = 3
+        out.append(m.decode_step_paged(torch.tensor([x, 7, x]), c))
+        assert c.held == [-1, 4, -1] and c.lengths.tolist() == [-1, 4, -1]
+    assert torch.equal(out[0], out[1]) and out[0].shape == (3, 50)
+
+
+@pytest.mark.parametrize("shape", [(1,), (2,), (4,), (3, 1), ()])
+def test_a_step_refuses_ids_of_another_shape(shape, plain_operators):
+    m, c = _model(), lm.PagedKVCache(CFG, 3, 6, page_size=16, device="cpu")
+    _begin(c, 1, 16)
+    with pytest.raises(ValueError, match="ids"):
+        m.decode_step_paged(torch.zeros(shape, dtype=torch.int64), c)
+    assert c.held == [-1, 16, -1] and len(c.free) == 5
