@@ -222,7 +222,7 @@ def device_status():
     kernel met a page number, length or position out of range.
 
     The launch whose wait ran out left its outputs unwritten, and what was out of range was left out; later launches ran
-    normally.  Reading clears the word."""
+    normally.  Reading clears what is reported; of both kinds the wait is reported first and the other by the next call."""
     code = C.c_int(0)
     st = load().flashmhf_device_status(C.byref(code))
     if st != 0:

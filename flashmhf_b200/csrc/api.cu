@@ -9,8 +9,8 @@
 
 namespace fmhf {
 
-// Per device: the status word (first failure wins) and the sequence number of the launch that failed.
-static __device__ int g_status_word;
+// Per device: the status word (first failure wins), the same for indices out of range, and the sequence number of the launch that failed.
+static __device__ int g_status_word, g_index_word;
 static __device__ unsigned g_abort_seq;
 
 namespace {
@@ -59,9 +59,10 @@ const DeviceCtl *device_ctl() {
     if (g_ctl_ready[dev].load(std::memory_order_acquire)) return &g_ctl[dev];
     std::lock_guard<std::mutex> lk(g_mu);
     if (!g_ctl_ready[dev].load(std::memory_order_relaxed)) {
-        void *ps = nullptr, *pa = nullptr;
+        void *ps = nullptr, *pi = nullptr, *pa = nullptr;
         int sms = 0;
         e = cudaGetSymbolAddress(&ps, g_status_word);
+        if (e == cudaSuccess) e = cudaGetSymbolAddress(&pi, g_index_word);
         if (e == cudaSuccess) e = cudaGetSymbolAddress(&pa, g_abort_seq);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess || sms < 1) {
@@ -69,6 +70,7 @@ const DeviceCtl *device_ctl() {
             return nullptr;
         }
         g_ctl[dev].status = static_cast<int *>(ps);
+        g_ctl[dev].index = static_cast<int *>(pi);
         g_ctl[dev].abort_seq = static_cast<unsigned *>(pa);
         g_ctl[dev].num_sms = sms;
         g_ctl[dev].device = dev;
@@ -572,18 +574,21 @@ int flashmhf_device_status(int *code) {
     if (code) *code = 0;
     const DeviceCtl *ctl = device_ctl();
     if (!ctl) return FLASHMHF_ERR_CUDA;
-    int *addr = ctl->status;
     cudaError_t e = cudaDeviceSynchronize();
-    int v = 0;
-    if (e == cudaSuccess) e = cudaMemcpy(&v, addr, sizeof(int), cudaMemcpyDeviceToHost);
-    if (e == cudaSuccess && v != 0) e = cudaMemset(addr, 0, sizeof(int));
+    // A call reports one word and clears that one: a wait that ran out first, an index out of range with the next call.
+    auto read = [&](int *word) {
+        int v = 0;
+        if (e == cudaSuccess) e = cudaMemcpy(&v, word, sizeof(int), cudaMemcpyDeviceToHost);
+        if (e == cudaSuccess && v != 0) e = cudaMemset(word, 0, sizeof(int));
+        return v;
+    };
+    const int timeout = read(ctl->status), index = timeout ? 0 : read(ctl->index);
     if (e != cudaSuccess) {
         set_cuda_error(e, "flashmhf_device_status");
         return FLASHMHF_ERR_CUDA;
     }
-    if (code) *code = v;
-    if (v >= kFirstIndexCode && v <= kLastIndexCode) return FLASHMHF_ERR_DEVICE_INDEX;
-    return v == 0 ? FLASHMHF_OK : FLASHMHF_ERR_DEVICE_TIMEOUT;
+    if (code) *code = timeout ? timeout : index;
+    return timeout ? FLASHMHF_ERR_DEVICE_TIMEOUT : index ? FLASHMHF_ERR_DEVICE_INDEX : FLASHMHF_OK;
 }
 
 }  // extern "C"

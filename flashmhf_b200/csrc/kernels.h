@@ -11,10 +11,12 @@ namespace fmhf {
 
 // Per-device control words and facts, resolved once per device (with that device current).
 //   status    : 0, or the code of the first bounded wait that ran out since the host last read it
+//   index     : 0, or the code of the first index out of range that a serving kernel met since then; a word of its own, so that
+//               neither report hides the other
 //   abort_seq : sequence number of the launch whose wait ran out; the other CTAs of THAT launch see it at
 //               their start and return at once, later launches (other numbers) run normally
 struct DeviceCtl {
-    int *status = nullptr;
+    int *status = nullptr, *index = nullptr;
     unsigned *abort_seq = nullptr;
     int num_sms = 0;
     int device = -1;
@@ -81,9 +83,6 @@ int paged_append(const flashmhf_paged_append_params &p, const DeviceCtl &ctl, cu
 size_t paged_attention_workspace_bytes(const flashmhf_paged_attention_params &p);
 int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &ctl, cudaStream_t st, int *n_launch);
 int prompt_attention(const flashmhf_prompt_attention_params &p, const DeviceCtl &ctl, cudaStream_t st, int *n_launch);
-// Status-word codes in this range name an index out of range, not a wait that ran out.
-constexpr int kFirstIndexCode = 400, kLastIndexCode = 599;
-
 // Launch.  `early`: with programmatic stream serialization, so that the kernel may start before the one ahead of it on the
 // stream has ended (as soon as that one's CTAs have all asked for it, or exited).
 // `cluster`: CTAs (along x) of a thread-block cluster.

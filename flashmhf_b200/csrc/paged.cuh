@@ -9,14 +9,14 @@
 
 namespace fmhf {
 
-// Codes of the status word for indices that only the device sees: all between kFirstIndexCode and kLastIndexCode.
+// Codes for indices that only the device sees (DeviceCtl::index).
 constexpr int kPagedAppendPage = 401, kPagedAppendPosition = 402, kPagedAppendRows = 403;
 constexpr int kPagedAttnPage = 501, kPagedAttnLength = 502;
 constexpr int kPromptRows = 551;
 
 constexpr int kMinScaleExp = -60;   // the smallest scale, 2^-60: what a page of zeros has
 
-__device__ __forceinline__ void note_index(int *status, int code) { atomicCAS(status, 0, code); }
+__device__ __forceinline__ void note_index(int *index, int code) { atomicCAS(index, 0, code); }
 
 // The smallest 2^n, n >= -60, with amax <= 448 * 2^n, by the bits of amax >= 0 (finite): 448 = 1.75 * 2^8.
 __device__ __forceinline__ float scale_for(uint32_t amax_bits) {

@@ -24,7 +24,7 @@ struct AppendArgs {
     long long q_tok, q_head, x_tok[2], x_head[2];
     __nv_bfloat16 *q_out, *k_out;
     const float *cos_t, *sin_t;
-    int *status;
+    int *index;
     int B, max_pages, num_pages, n_kv, tokens, n_q, max_pos;
     unsigned page_blocks;    // blocks of the first kind
 };
@@ -130,7 +130,7 @@ __device__ __forceinline__ Piece piece_of(const AppendArgs &a, int b) {
     p.first = a.cu ? __ldg(a.cu + b) : b;
     p.last = a.cu ? __ldg(a.cu + b + 1) : b + 1;
     if (p.first < 0 || p.last > a.tokens || p.last < p.first) {
-        note_index(a.status, kPagedAppendRows);
+        note_index(a.index, kPagedAppendRows);
         p.first = p.last = 0;
     }
     if (p.before < 0) p.last = p.first;
@@ -177,10 +177,10 @@ __device__ void append_page(const AppendArgs &a, int log2_p, uint32_t *red) {
     }
     const int page = page_no < a.max_pages ? __ldg(a.table + b * a.table_stride + page_no) : -1;
     if (page < 0 || page >= a.num_pages) {
-        if (threadIdx.x == 0) note_index(a.status, kPagedAppendPage);
+        if (threadIdx.x == 0) note_index(a.index, kPagedAppendPage);
         return;
     }
-    if (threadIdx.x == 0 && min((long long)P, end - start) > row_end) note_index(a.status, kPagedAppendPosition);
+    if (threadIdx.x == 0 && min((long long)P, end - start) > row_end) note_index(a.index, kPagedAppendPosition);
     float *sp = a.scale[which] + (long long)page * a.n_kv + head;
     const float old = had > 0 ? *sp : 0.f;
     float y1[KEEP ? PASSES : 1][PAIRS], y2[KEEP ? PASSES : 1][PAIRS];
@@ -272,7 +272,7 @@ __device__ void append_token(const AppendArgs &a, int log2_p) {
     const int P = 1 << log2_p, page_no = pos >> log2_p, row = pos & (P - 1);
     const int page = page_no < a.max_pages ? __ldg(a.table + b * a.table_stride + page_no) : -1;
     if (page < 0 || page >= a.num_pages || pos >= a.max_pos) {
-        note_index(a.status, page < 0 || page >= a.num_pages ? kPagedAppendPage : kPagedAppendPosition);
+        note_index(a.index, page < 0 || page >= a.num_pages ? kPagedAppendPage : kPagedAppendPosition);
         return;
     }
     float *sp = a.scale[which] + (long long)page * a.n_kv + head;
@@ -337,7 +337,7 @@ __device__ void append_queries(const AppendArgs &a) {
     const long long pos = position_of(a, (int)t);
     if (pos < 0) return;
     if (pos >= a.max_pos) {
-        note_index(a.status, kPagedAppendPosition);
+        note_index(a.index, kPagedAppendPosition);
         return;
     }
     float c[PAIRS], s[PAIRS];
@@ -386,7 +386,7 @@ int paged_append(const flashmhf_paged_append_params &p, const DeviceCtl &ctl, cu
     a.q_out = static_cast<__nv_bfloat16 *>(p.q_out);
     a.k_out = static_cast<__nv_bfloat16 *>(p.k_out);
     a.cos_t = p.cos_t; a.sin_t = p.sin_t;
-    a.status = ctl.status;
+    a.index = ctl.index;
     a.B = p.seq.B; a.max_pages = p.seq.max_pages; a.num_pages = g.num_pages; a.n_kv = g.n_kv;
     a.tokens = p.tokens; a.n_q = p.q ? p.n_q : 0; a.max_pos = p.max_positions;
     const int P = g.page_size, threads = a.cu ? (P * 8 < 256 ? P * 8 : 256) : 128;

@@ -63,7 +63,7 @@ struct PagedArgs {
     float *part;                     // [worker][2][kCols][HD] sums of a warp's parts
     float2 *ml;                      // [worker][2][kCols] their maxima and sums of weights
     int4 *shared_by;                 // [item]: first and last worker of it, and which part of the first one's
-    int *status;
+    int *index;
     int B, max_pages, num_pages, n_kv, n_q, n_new, log_page, group, col_tiles, workers;
     float c;                         // scale * log2(e)
     WaitArgs wait;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[W]) {
 __device__ __forceinline__ int length_of(const PagedArgs &a, int b) {
     const int n = __ldg(a.lengths + b);
     const long long most = (long long)a.max_pages << a.log_page;
-    if (n > most) note_index(a.status, kPagedAttnLength);
+    if (n > most) note_index(a.index, kPagedAttnLength);
     return max(0, (int)min((long long)n, most));
 }
 __device__ __forceinline__ long long units_of(int len) { return (len + kUnit - 1) / kUnit; }
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<HD>::kBlocks) paged_attentio
         auto pages = [&](int first, int &pid, float &k, float &v) {
             pid = first + lane <= last_page ? __ldg(table + first + lane) : -1;
             if (first + lane <= last_page && (pid < 0 || pid >= a.num_pages)) {
-                note_index(a.status, kPagedAttnPage);
+                note_index(a.index, kPagedAttnPage);
                 pid = -1;
             }
             const long long at = (long long)max(pid, 0) * a.n_kv + head;      // (of no page: any scale)
@@ -588,7 +588,7 @@ int paged_attention(const flashmhf_paged_attention_params &p, const DeviceCtl &c
     a.lengths = p.seq.lengths; a.table = p.seq.table; a.table_stride = p.seq.table_stride;
     a.q = static_cast<const __nv_bfloat16 *>(p.q); a.o = static_cast<__nv_bfloat16 *>(p.o);
     for (int i = 0; i < 3; ++i) { a.q_stride[i] = p.q_stride[i]; a.o_stride[i] = p.o_stride[i]; }
-    a.lse = p.lse; a.status = ctl.status;
+    a.lse = p.lse; a.index = ctl.index;
     a.B = p.seq.B; a.max_pages = p.seq.max_pages; a.num_pages = g.num_pages; a.n_kv = g.n_kv; a.n_q = p.n_q; a.n_new = p.n_new;
     a.log_page = g.page_size == 16 ? 4 : g.page_size == 32 ? 5 : g.page_size == 64 ? 6 : 7;
     a.group = p.n_q / g.n_kv;

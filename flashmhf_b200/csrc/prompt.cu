@@ -90,6 +90,7 @@ struct PromptArgs {
     // scale log2(e) is c * before, c > 0: scores are multiplied by `before` as they come, and by c in the exponent, behind the mask.  `before` is the sign,
     // but where |scale| log2(e) is below 2^-60 it is all of it and c is 1: a c of 0 would make no number of a masked score's -inf.
     float c, before;
+    int *index;
     WaitArgs wait;
 };
 
@@ -106,7 +107,7 @@ __device__ __forceinline__ bool prompt_item(const PromptArgs &a, int index, Prom
     }
     const int q0 = __ldg(a.cu_q + lo), q1 = __ldg(a.cu_q + lo + 1), k0 = __ldg(a.cu_k + lo), k1 = __ldg(a.cu_k + lo + 1);
     if (q0 < 0 || q1 > a.tokens_q || q1 < q0 || k0 < 0 || k1 > a.tokens_k || k1 < k0) {
-        note_index(a.wait.status, kPromptRows);
+        note_index(a.index, kPromptRows);
         return false;
     }
     const int r0 = (slot - (q0 / kRows + lo)) * kRows, lq = q1 - q0, lk = k1 - k0;
@@ -644,6 +645,7 @@ int prompt_attention(const flashmhf_prompt_attention_params &p, const DeviceCtl 
     const bool tiny = size < 0x1p-60f;
     a.c = tiny ? 1.f : size;
     a.before = tiny ? c : c < 0.f ? -1.f : 1.f;
+    a.index = ctl.index;
     a.wait = wait_args(&ctl);
     switch (p.head_dim) {
         case 64: return launch_prompt<64>(p, a, ctl.device, st, n_launch);

@@ -356,8 +356,9 @@ int flashmhf_prompt_attention(const flashmhf_prompt_attention_params *p, void *s
  * launches are not affected: they run normally whether or not the word has been read.  Because the
  * entry points only enqueue work they cannot report the condition themselves; call this wherever the
  * host already synchronises (after reading back a loss, at the end of a step).
- * The serving kernels use the same word for what they can see on the device alone: a page number, length or position out of range
- * is left out (nothing is read or written there), and the call returns FLASHMHF_ERR_DEVICE_INDEX with the kernel's code.
+ * The serving kernels have a second word for what they can see on the device alone: a page number, length or position out of range
+ * is left out (nothing is read or written there), and the call returns FLASHMHF_ERR_DEVICE_INDEX with the kernel's code.  A call reads and
+ * clears one word: where a wait has run out as well, that is reported first and the index by the next call.
  * Reference counterpart: none. */
 int flashmhf_device_status(int *code);
 

@@ -94,3 +94,21 @@ def test_paged_attention_pages_of_very_different_scales(hd, ratio, order):
         q = (torch.randn(1, G, hd, generator=g) * size).bfloat16()
         o = fm.paged_attention(q.cuda(), pages, ref.ints([n]), ref.ints([list(range(10))]))
         _strict(o[0], *_one_head(q[0], K, V, hd ** -0.5))
+
+
+def test_a_wait_that_runs_out_is_reported_before_an_index_out_of_range():
+    """Both in one run, in either order: neither report hides the other."""
+    import flashmhf_b200 as fm
+    from flashmhf_b200 import _lib
+    lib, stream = _lib.load(), C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    pages, q = _pool(3, 1, 16, 64, 0), _packed(1, 2, 64, 0).cuda()
+    steps = (lambda: fm.paged_attention(q, pages, ref.ints([20]), ref.ints([[0, 7]])),
+             lambda: lib.flashmhf_selftest_bounded_wait(2_000_000, stream))
+    for order in ((0, 1), (1, 0)):
+        for i in order:
+            steps[i]()
+        for status in (-9, -11):
+            with pytest.raises(_lib.FlashMHFError) as e:
+                fm.check_device_status()
+            assert e.value.status == status
+        fm.check_device_status()
