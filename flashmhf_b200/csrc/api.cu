@@ -580,8 +580,12 @@ int flashmhf_device_status(int *code) {
         int v = 0;
         if (e == cudaSuccess) e = cudaMemcpy(&v, word, sizeof(int), cudaMemcpyDeviceToHost);
         if (e == cudaSuccess && v != 0) e = cudaMemset(word, 0, sizeof(int));
+        if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(nullptr);      // (a launch on another stream may come right after this call)
         return v;
     };
+    // A captured launch keeps its number in every replay: the number of the one that gave up goes together with the report of it (and before it: whatever
+    // fails here, a launch that is left out has a code in the status word).
+    if (e == cudaSuccess) e = cudaMemset(ctl->abort_seq, 0, sizeof(unsigned));
     const int timeout = read(ctl->status), index = timeout ? 0 : read(ctl->index);
     if (e != cudaSuccess) {
         set_cuda_error(e, "flashmhf_device_status");

@@ -14,7 +14,8 @@ namespace fmhf {
 //   index     : 0, or the code of the first index out of range that a serving kernel met since then; a word of its own, so that
 //               neither report hides the other
 //   abort_seq : sequence number of the launch whose wait ran out; the other CTAs of THAT launch see it at
-//               their start and return at once, later launches (other numbers) run normally
+//               their start and return at once, later launches (other numbers) run normally.  A captured launch has one
+//               number for all its replays: those return at once too, until the host reads the status word, which clears this
 struct DeviceCtl {
     int *status = nullptr, *index = nullptr;
     unsigned *abort_seq = nullptr;

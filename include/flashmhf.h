@@ -353,7 +353,9 @@ int flashmhf_prompt_attention(const flashmhf_prompt_attention_params *p, void *s
  * Semantics of a run-out wait: every mbarrier wait in the kernels is bounded (about 1.5 s); the launch
  * whose wait ran out returns early through its normal teardown and leaves its outputs UNWRITTEN, its
  * remaining CTAs drain at once, and the first code is kept in the word until this call reads it.  Later
- * launches are not affected: they run normally whether or not the word has been read.  Because the
+ * launches are not affected: they run normally whether or not the word has been read.  (Replays of a captured
+ * launch whose wait ran out count as that launch: they are left out until this call has read the word, and run
+ * normally after it.)  Because the
  * entry points only enqueue work they cannot report the condition themselves; call this wherever the
  * host already synchronises (after reading back a loss, at the end of a step).
  * The serving kernels have a second word for what they can see on the device alone: a page number, length or position out of range

@@ -112,3 +112,25 @@ def test_a_wait_that_runs_out_is_reported_before_an_index_out_of_range():
                 fm.check_device_status()
             assert e.value.status == status
         fm.check_device_status()
+
+
+def test_a_captured_launch_that_gave_up_reports_each_time():
+    """A captured launch keeps its number: what the status call has read does not keep the next replay from running, or from saying that it gave up."""
+    from flashmhf_b200 import _lib
+    lib = _lib.load()
+    _lib.device_status()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert lib.flashmhf_selftest_bounded_wait(2_000_000, C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    _lib.device_status()
+    for _ in range(3):
+        graph.replay()
+        with pytest.raises(_lib.FlashMHFError) as e:
+            _lib.device_status()
+        assert e.value.status == -9 and e.value.code == _lib.SELFTEST_CODE
+        _lib.device_status()
+    graph.replay()
+    graph.replay()               # before anyone has read of the first
+    with pytest.raises(_lib.FlashMHFError):
+        _lib.device_status()
+    _lib.device_status()
