@@ -824,7 +824,7 @@ bool rows_ok(const Tensor &t) {
         if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
     return true;
 }
-Tensor rows(const Tensor &t) { return rows_ok(t) ? t : t.contiguous(); }
+Tensor rows(const Tensor &t) { return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }      // (a contiguous tensor may lie off a 16-byte boundary)
 void strides_of(const Tensor &t, int64_t *to) {   // of all but the innermost dimension; one of extent 1 has none that matters
     for (int64_t i = 0; i + 1 < t.dim(); ++i) to[i] = t.size(i) > 1 ? t.stride(i) : 0;
 }

@@ -134,3 +134,27 @@ def test_a_captured_launch_that_gave_up_reports_each_time():
     with pytest.raises(_lib.FlashMHFError):
         _lib.device_status()
     _lib.device_status()
+
+
+def _shifted(x):
+    """The same contiguous tensor two bytes behind a 16-byte boundary."""
+    y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape)
+    y.copy_(x)
+    assert y.is_contiguous() and y.data_ptr() % 16 != 0
+    return y
+
+
+def test_inputs_off_a_16_byte_boundary():
+    import flashmhf_b200 as fm
+    q, k, v = (_packed(40, h, 64, i).cuda() for i, h in enumerate((4, 2, 2)))
+    cu, cos, sin = ref.ints([0, 17, 40]), *ref.tables(64, 64)
+    args = (cos, sin, ref.ints([0, 0]), ref.ints([[0, 1], [2, 3]]))
+    runs = []
+    for f in (lambda x: x, _shifted):
+        pages = fm.KVPages.empty(4, 2, 32, 64)
+        for t in pages[:2]:
+            t.view(torch.uint8).zero_()
+        qr, kr = fm.paged_append(pages, f(k), f(v), *args, q=f(q), cu_seqlens=cu, rotated_keys=True)
+        runs.append([qr, kr, *(t.view(torch.uint8) for t in pages), fm.prompt_attention(f(q), f(k), f(v), cu),
+                     fm.paged_attention(f(q[:2].clone()), pages, ref.ints([17, 23]), args[3])])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
