@@ -828,6 +828,11 @@ Tensor rows(const Tensor &t) { return rows_ok(t) ? t : t.clone(at::MemoryFormat:
 void strides_of(const Tensor &t, int64_t *to) {   // of all but the innermost dimension; one of extent 1 has none that matters
     for (int64_t i = 0; i + 1 < t.dim(); ++i) to[i] = t.size(i) > 1 ? t.stride(i) : 0;
 }
+// A call writes these in place, below autograd: a graph that has saved one of them has to notice.
+void written(std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 Tensor given_or_new(const std::optional<Tensor> &out, const Tensor &like) {
     if (!out) return at::empty(like.sizes(), like.options());
     if (out->sizes() != like.sizes() || out->scalar_type() != like.scalar_type() || out->device() != like.device() || !rows_ok(*out))
@@ -899,7 +904,7 @@ std::pair<std::optional<Tensor>, std::optional<Tensor>> paged_append(const Tenso
             throw py::value_error("cos and sin must be contiguous fp32 [positions, " + std::to_string(hd / 2) + "]");
     const Tensor none, &q1 = q0 ? *q0 : none;
     same_device("paged_append", kp, {&vp, &ks, &vs, &k0, &v0, &cos_t, &sin_t, &lengths, &table0, &q1, &cu});
-    no_gradients("paged_append", {&k0, &v0, &cos_t, &sin_t, &q1, &ks, &vs});
+    no_gradients("paged_append", {&k0, &v0, &cos_t, &sin_t, &q1, &kp, &vp, &ks, &vs});
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(kp.device());
     const Tensor k = rows(k0), v = rows(v0), q = q0 ? rows(*q0) : Tensor();
@@ -924,6 +929,7 @@ std::pair<std::optional<Tensor>, std::optional<Tensor>> paged_append(const Tenso
     p.tokens = (int32_t)T;
     p.max_positions = (int32_t)std::min<int64_t>(cos_t.size(0), INT32_MAX);
     check(api.paged_append(&p, current_stream(kp)));
+    written({&kp, &vp, &ks, &vs});
     return {q_out, k_out};
 }
 
@@ -946,7 +952,7 @@ Attended paged_attention(const Tensor &q0, const Tensor &kp, const Tensor &vp, c
     const Tensor table = B ? table_rows(table0, B, p.pages.page_size) : table0;
     p.scale = softmax_scale(scale, hd);
     same_device("paged_attention", q0, {&kp, &vp, &ks, &vs, &lengths, &table0});
-    no_gradients("paged_attention", {&q0, &ks, &vs});
+    no_gradients("paged_attention", {&q0, &kp, &vp, &ks, &vs});
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(q0.device());
     const Tensor q = rows(q0);
@@ -973,6 +979,7 @@ Attended paged_attention(const Tensor &q0, const Tensor &kp, const Tensor &vp, c
         p.workspace = ws.data_ptr();
     }
     check(api.paged_attention(&p, current_stream(q0)));
+    if (out) written({&o});
     return with_lse(o, lse);
 }
 
@@ -1014,6 +1021,7 @@ Attended prompt_attention(const Tensor &q0, const Tensor &k0, const Tensor &v0, 
     p.B = (int32_t)B; p.tokens_q = (int32_t)T; p.tokens_k = (int32_t)Tk; p.n_q = (int32_t)n_q; p.n_kv = (int32_t)n_kv; p.head_dim = (int32_t)hd;
     p.causal = causal ? 1 : 0;
     check(api.prompt_attention(&p, current_stream(q0)));
+    if (out) written({&o});
     return with_lse(o, lse);
 }
 

@@ -158,3 +158,31 @@ def test_inputs_off_a_16_byte_boundary():
         runs.append([qr, kr, *(t.view(torch.uint8) for t in pages), fm.prompt_attention(f(q), f(k), f(v), cu),
                      fm.paged_attention(f(q[:2].clone()), pages, ref.ints([17, 23]), args[3])])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_what_is_written_in_place_has_a_new_version():
+    import flashmhf_b200 as fm
+    pages, x = fm.KVPages.empty(2, 2, 16, 64), _packed(3, 2, 64, 0).cuda()
+    cos, sin = ref.tables(16, 64)
+    was = [t._version for t in pages]
+    fm.paged_append(pages, x, x, cos, sin, ref.ints([0]), ref.ints([[0]]), cu_seqlens=ref.ints([0, 3]))
+    assert all(t._version > w for t, w in zip(pages, was))
+    for call in (lambda out: fm.paged_attention(x[:1], pages, ref.ints([3]), ref.ints([[0]]), out=out[:1]),
+                 lambda out: fm.prompt_attention(x, x, x, ref.ints([0, 3]), out=out)):
+        out = torch.empty_like(x)
+        was, still = out._version, x._version
+        call(out)
+        assert out._version > was and x._version == still
+    with torch.inference_mode():          # (tensors that count no versions)
+        fm.prompt_attention(x, x, x, ref.ints([0, 3]), out=torch.empty_like(x))
+    scale = torch.ones(1, device="cuda", requires_grad=True)
+    saved = (scale * pages.k_scale).sum()            # keeps k_scale for the gradient of `scale`
+    with torch.no_grad():
+        fm.paged_append(pages, x[:1], x[:1], cos, sin, ref.ints([3]), ref.ints([[0]]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    grad = pages._replace(k=pages.k.detach().requires_grad_())
+    for call in (lambda: fm.paged_append(grad, x[:1], x[:1], cos, sin, ref.ints([3]), ref.ints([[0]])),
+                 lambda: fm.paged_attention(x[:1], grad, ref.ints([3]), ref.ints([[0]]))):
+        with pytest.raises(NotImplementedError):
+            call()
