@@ -17,8 +17,10 @@
 #include <dlfcn.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
+#include <vector>
 
 #include "../../include/flashmhf.h"
 
@@ -833,8 +835,45 @@ void written(std::initializer_list<const Tensor *> ts) {
     for (const Tensor *t : ts)
         if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
+// Elements from the first to behind the last one of the dimensions from `from` on (of a tensor with elements).
+int64_t extent(const Tensor &t, int64_t from) {
+    int64_t n = 1;
+    for (int64_t i = from; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+    return n;
+}
+// Do two bf16 tensors share memory?  Exact for views of one projection (the same outermost stride, a row of either shorter than it); other tensors
+// whose ranges meet count as sharing.
+bool share(const Tensor &a, const Tensor &b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const int64_t d = (reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr())) / 2;
+    if (d >= extent(a, 0) || -d >= extent(b, 0)) return false;
+    const int64_t s = a.stride(0), ea = extent(a, 1), eb = extent(b, 1);
+    if (a.size(0) < 2 || b.size(0) < 2 || s != b.stride(0) || ea > s || eb > s) return true;
+    const int64_t at = ((d % s) + s) % s;
+    return at < ea || at + eb > s;
+}
+// No element twice: each dimension steps over all of those with smaller strides.
+bool distinct(const Tensor &t) {
+    std::vector<std::pair<int64_t, int64_t>> dims;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t n = 1;
+    for (const auto &[stride, size] : dims) {
+        if (stride < n) return false;
+        n = stride * (size - 1) + n;
+    }
+    return true;
+}
+// `o` may take the place of the queries, of which each block has read its own rows when it writes them; nothing else that is read.
+void apart(const Tensor &o, const Tensor &q, std::initializer_list<const Tensor *> others) {
+    bool ok = !share(o, q) || (o.data_ptr() == q.data_ptr() && o.strides() == q.strides());
+    for (const Tensor *t : others) ok = ok && !share(o, *t);
+    if (!ok) throw py::value_error("out must not share memory with the inputs, but for taking the place of all of q");
+}
 Tensor given_or_new(const std::optional<Tensor> &out, const Tensor &like) {
     if (!out) return at::empty(like.sizes(), like.options());
+    if (!distinct(*out)) throw py::value_error("out must not have an element twice");
     if (out->sizes() != like.sizes() || out->scalar_type() != like.scalar_type() || out->device() != like.device() || !rows_ok(*out))
         throw py::value_error("out must be like q, its last dimension contiguous and the others in steps of 16 bytes");
     TORCH_CHECK_NOT_IMPLEMENTED(!out->requires_grad(), "out must not require gradients");
@@ -958,6 +997,7 @@ Attended paged_attention(const Tensor &q0, const Tensor &kp, const Tensor &vp, c
     const Tensor q = rows(q0);
     const Tensor o = given_or_new(out, q0), lse = want_lse ? at::empty(q0.sizes().slice(0, dim - 1), q0.options().dtype(at::kFloat)) : Tensor();
     if (B == 0) return with_lse(o, lse);
+    if (out) apart(o, q, {});
     p.seq = sequences_of(lengths, table);
     p.q = q.data_ptr(); p.o = o.data_ptr();
     if (dim == 4) {
@@ -1007,6 +1047,7 @@ Attended prompt_attention(const Tensor &q0, const Tensor &k0, const Tensor &v0, 
     const Tensor o = given_or_new(out, q0), lse = want_lse ? at::empty({T, n_q}, q0.options().dtype(at::kFloat)) : Tensor();
     if (T == 0 || B == 0) return with_lse(o, lse);
     if (T > INT32_MAX || Tk > INT32_MAX) throw py::value_error("more than 2^31 tokens in a call");
+    if (out) apart(o, q, {&k, &v});
     // (no keys at all: the kernel still writes zeros, and reads none of the one row that it is told of)
     p.q = q.data_ptr(); p.o = o.data_ptr();
     p.k = Tk ? k.data_ptr() : q.data_ptr(); p.v = Tk ? v.data_ptr() : q.data_ptr();

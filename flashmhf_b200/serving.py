@@ -65,7 +65,7 @@ def paged_attention(q, pages, lengths, page_table, scale=None, out=None, return_
     q [B, n_q, head_dim] (one token a sequence) or [B, n_new, n_q, head_dim] with n_new up to 16, rotated and already appended;
     ``lengths`` int32 [B]: positions in the cache, those of the new tokens included (new token i sees the first
     lengths - (n_new - 1 - i)); n_q a multiple of n_kv.  ``scale`` defaults to head_dim ** -0.5.  A row that sees nothing gives
-    zeros.  ``return_lse``: also the natural logarithm of the sum of exponentials, fp32, q's shape without the last dimension
+    zeros.  ``out``: like q, its last dimension contiguous and the others in steps of 16 bytes; it may be q itself.  ``return_lse``: also the natural logarithm of the sum of exponentials, fp32, q's shape without the last dimension
     (-inf for a row that sees nothing): what parts of a longer attention are merged with.  Rows of a page behind a sequence's length are
     never used, whatever they hold; a value of a later new token that is not a finite number also reaches the new tokens before it."""
     o, lse = _lib.native().paged_attention(q, pages.k, pages.v, pages.k_scale, pages.v_scale, lengths, page_table, scale, out, return_lse)
@@ -77,7 +77,8 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
 
     Rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of q belong to sequence b, and those of ``cu_seqlens_k`` (default: the same) of k and
     v; int32 [B+1] on the device.  Causal: the last row sees all keys of its sequence, each row before it one less; a row that
-    sees nothing gives zeros.  Rows of no sequence are left as they are (in a new output: undefined).  ``return_lse`` as for
+    sees nothing gives zeros.  Rows of no sequence are left as they are (in a new output: undefined).  ``out`` as for ``paged_attention``; it must
+    not lie over k or v.  ``return_lse`` as for
     ``paged_attention``, [T, n_q].  Sequences do not touch each other, whatever their neighbours hold; within a sequence the mask gives
     weights of zero, so that a value which is not a finite number also reaches up to 127 rows before its own."""
     o, lse = _lib.native().prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, out, return_lse)

@@ -186,3 +186,29 @@ def test_what_is_written_in_place_has_a_new_version():
                  lambda: fm.paged_attention(x[:1], grad, ref.ints([3]), ref.ints([[0]]))):
         with pytest.raises(NotImplementedError):
             call()
+
+
+def test_outputs_that_lie_over_inputs():
+    """The output may take the queries' place; over keys, values or itself it is refused."""
+    import flashmhf_b200 as fm
+    qkv = _packed(150, 6, 64, 5).cuda()
+    cu = ref.ints([0, 20, 150])
+    parts = lambda t: (t[:, :2], t[:, 2:4], t[:, 4:])  # noqa: E731
+    want = fm.prompt_attention(*parts(qkv), cu)
+    x = qkv.clone()
+    assert torch.equal(fm.prompt_attention(*parts(x), cu, out=parts(x)[0]), want) and torch.equal(x[:, 2:], qkv[:, 2:])
+    q, k, v = (t.contiguous() for t in parts(qkv))
+    for out in (k, v, torch.empty(150 * 64 + 128, dtype=torch.bfloat16, device="cuda").as_strided((150, 2, 64), (64, 64, 1))):
+        with pytest.raises(ValueError):
+            fm.prompt_attention(q, k, v, cu, out=out)
+    for bad in parts(x)[1:]:
+        with pytest.raises(ValueError):
+            fm.prompt_attention(*parts(x), cu, out=bad)
+    assert torch.equal(k, parts(qkv)[1]) and torch.equal(v, parts(qkv)[2])
+    pages = _pool(4, 2, 32, 64, 0)
+    q1 = q[:2].clone()
+    args = (pages, ref.ints([30, 50]), ref.ints([[0, 1], [2, 3]]))
+    for t in pages[:2]:
+        t.view(torch.uint8).copy_(torch.randn(t.shape).to(torch.float8_e4m3fn).view(torch.uint8))
+    want = fm.paged_attention(q1, *args)
+    assert torch.equal(fm.paged_attention(q1, *args, out=q1), want)
