@@ -416,9 +416,12 @@ class PagedKVCache:
 
     def release(self, b):
         """Sequence ``b`` ends: its pages may go to others."""
+        if not 0 <= b < len(self.held):
+            raise ValueError(f"place {b} is not one of the cache's {len(self.held)}")
         self.free += self.owned[b][::-1]
         self.owned[b], self.held[b] = [], -1
         self.lengths[b] = -1
+        self.table[b] = -1        # (a replayed step for which nobody has called `reserve` meets no page, not one that is another's by now)
 
     def nbytes(self):
         """Bytes of keys, values and scales that a step over what the cache holds reads."""
@@ -512,17 +515,19 @@ class DecoderLM(nn.Module):
                 raise ValueError(f"place {b} of the cache holds a sequence: release it first")
             if prompts[b].dim() != 1 or prompts[b].numel() == 0:
                 raise ValueError("a prompt is a 1-D tensor of at least one id")
+        if not places:
+            return self.lm_head.weight.new_empty(0, self.cfg.vocab_size)
         counts = [prompts[b].numel() if b in prompts else 0 for b in range(len(cache.held))]
         cache.reserve(counts)
         device = cache.table.device
         starts = [0]
         for n in counts:
             starts.append(starts[-1] + n)
-        cu = torch.tensor(starts, dtype=torch.int32, device=device)
-        at = torch.tensor(places, device=device)
-        ids = torch.cat([prompts[b].to(device) for b in places])
-        cache.lengths[at] = 0
         try:
+            cu = torch.tensor(starts, dtype=torch.int32, device=device)
+            at = torch.tensor(places, device=device)
+            ids = torch.cat([prompts[b].to(device) for b in places])
+            cache.lengths[at] = 0
             h = self._paged(ids[None], cache, None, cu)[0]
         except BaseException:
             for b in places:

@@ -38,3 +38,32 @@ def test_a_step_refuses_ids_of_another_shape(shape, plain_operators):
     with pytest.raises(ValueError, match="ids"):
         m.decode_step_paged(torch.zeros(shape, dtype=torch.int64), c)
     assert c.held == [-1, 16, -1] and len(c.free) == 5
+
+
+def test_release_forgets_the_pages_and_refuses_places_outside_the_batch():
+    """Another sequence may own them: a step that is replayed without `reserve` must meet no page there, not somebody else's."""
+    c = lm.PagedKVCache(CFG, 3, 6, page_size=16, max_len=64, device="cpu")
+    _begin(c, 0, 40)
+    _begin(c, 2, 17)
+    for b in (-1, 3, -3):
+        with pytest.raises(ValueError, match="place"):
+            c.release(b)
+    assert c.held == [40, -1, 17] and len(c.free) == 1 and [len(o) for o in c.owned] == [3, 0, 2]
+    c.release(0)
+    assert c.table[0].tolist() == [-1] * 4 and c.table[2, :2].tolist() == c.owned[2] and len(c.free) == 4
+    c.release(0)                      # (of a place that is free already: nothing)
+    assert c.held == [-1, -1, 17] and len(c.free) == 4
+
+
+def test_a_prefill_of_nothing_and_one_that_fails_half_way(plain_operators):
+    m, c = _model(), lm.PagedKVCache(CFG, 3, 6, page_size=16, max_len=64, device="cpu")
+    _begin(c, 0, 20)
+    empty = m.prefill_paged({}, c)
+    assert empty.shape == (0, 50) and empty.dtype == m.lm_head.weight.dtype and c.held == [20, -1, -1] and len(c.free) == 4
+    good = torch.arange(5)
+    for bad in (torch.zeros(40, dtype=torch.int64, device="meta"), torch.full((40,), 99)):      # no data to copy; no such token
+        with pytest.raises(Exception):
+            m.prefill_paged({1: good, 2: bad}, c)
+        assert c.held == [20, -1, -1] and c.owned[1:] == [[], []] and len(c.free) == 4 and c.lengths[1:].tolist() == [-1, -1]
+        assert bool((c.table[1:] == -1).all())
+    assert m.prefill_paged({2: good}, c).shape == (1, 50) and c.held == [20, -1, 5]
