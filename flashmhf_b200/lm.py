@@ -14,6 +14,7 @@ no CPU stand-in for it in this package.
 """
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
@@ -166,12 +167,15 @@ class Attention(nn.Module):
         self.v_proj = nn.Linear(cfg.hidden_size, self.nkv * self.hd, bias=False)
         self.o_proj = nn.Linear(self.nh * self.hd, cfg.hidden_size, bias=False)
 
-    def forward(self, x, cos, sin, kv_out=None, link=None, tables=None):
-        """``tables``: optional fp32 halves of cos and sin (lm_ops.rotary_tables_f32), made once for all layers.
+    def forward(self, x, cos, sin, kv_out=None, link=None, tables=None, paged=None):
+        """``paged``: optional Paged: x are new tokens of a paged cache's sequences, and ``paged`` below is what is done (cos and sin are not used).
+        ``tables``: optional fp32 halves of cos and sin (lm_ops.rotary_tables_f32), made once for all layers.
         ``kv_out``: optional (k_cache, v_cache) of one layer, [B, n_kv, T_max, hd]; the keys (rotated) and values of
         the S positions are stored at [0, S) for later ``decode`` calls.
         ``link``: optional SequenceLink when a sequence is split over two ranks: the rank with the earlier part sends
         its keys and values on, the rank with the later part receives them and attends over both parts."""
+        if paged is not None:
+            return self.paged(x, *paged)
         B, S, _ = x.shape
         if tables is not None and kv_out is None and link is None and x.is_cuda and x.dtype == torch.bfloat16 and self.hd % 16 == 0 and \
                 not torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda"):
@@ -274,21 +278,15 @@ class DecoderLayer(nn.Module):
         self.input_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
 
-    def forward(self, h, cos, sin, kv_out=None, link=None):
-        h, d = self.step(h, None, cos, sin, kv_out, link)
+    def forward(self, h, cos, sin, kv_out=None, link=None, paged=None):
+        h, d = self.step(h, None, cos, sin, kv_out, link, paged=paged)
         return h + d
 
-    def step(self, h, d, cos, sin, kv_out=None, link=None, tables=None):
+    def step(self, h, d, cos, sin, kv_out=None, link=None, tables=None, paged=None):
         """The layer on h + d (the residual stream and what the layer before has yet to add to it); returns the new pair, so
         that every addition happens in the norm that follows it, across layers too."""
         h, x = add_norm(self.input_layernorm, h, d)
-        h, x = add_norm(self.post_attention_layernorm, h, self.self_attn(x, cos, sin, kv_out, link, tables))
-        return h, self.mlp(x)
-
-    def paged(self, h, d, pages, cache, lengths, cu=None):
-        """The layer on h + d with a paged cache (see ``step`` and Attention.paged); returns the new pair."""
-        h, x = add_norm(self.input_layernorm, h, d)
-        h, x = add_norm(self.post_attention_layernorm, h, self.self_attn.paged(x, pages, cache, lengths, cu))
+        h, x = add_norm(self.post_attention_layernorm, h, self.self_attn(x, cos, sin, kv_out, link, tables, **({} if paged is None else {"paged": paged})))
         return h, self.mlp(x)
 
     def decode(self, h, cos_p, sin_p, k_cache, v_cache, pos):
@@ -302,6 +300,14 @@ class _Body(nn.Module):
         self.embed_tokens = nn.Embedding(cfg.vocab_size, cfg.hidden_size)
         self.layers = nn.ModuleList(DecoderLayer(cfg, ffn) for _ in range(cfg.num_hidden_layers))
         self.norm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
+
+
+class Paged(NamedTuple):
+    """What a layer is given in a pass over a PagedKVCache: its pages, the cache, and the arguments of Attention.paged."""
+    pages: tuple
+    cache: object
+    lengths: torch.Tensor
+    cu: torch.Tensor
 
 
 class SequenceLink:
@@ -500,7 +506,11 @@ class DecoderLM(nn.Module):
     def _paged(self, ids, cache, lengths, cu=None):
         h, d = self.model.embed_tokens(ids), None
         for layer, pages in zip(self.model.layers, cache.pools):
-            h, d = layer.paged(h, d, pages, cache, lengths, cu)
+            paged = Paged(pages, cache, lengths, cu)
+            if _as_written(layer, DecoderLayer):
+                h, d = layer.step(h, d, None, None, paged=paged)
+            else:
+                h, d = layer(h if d is None else h + d, None, None, paged=paged), None
         return add_norm(self.model.norm, h, d)[1]
 
     @torch.no_grad()

@@ -67,3 +67,35 @@ def test_a_prefill_of_nothing_and_one_that_fails_half_way(plain_operators):
         assert c.held == [20, -1, -1] and c.owned[1:] == [[], []] and len(c.free) == 4 and c.lengths[1:].tolist() == [-1, -1]
         assert bool((c.table[1:] == -1).all())
     assert m.prefill_paged({2: good}, c).shape == (1, 50) and c.held == [20, -1, 5]
+
+
+class _Wrapped(torch.nn.Module):
+    """Another module around one, as checkpointing or sharding puts it in place."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, *a, **k):
+        return self.inner(*a, **k)
+
+
+def _serve(m):
+    c = lm.PagedKVCache(CFG, 2, 6, page_size=16, device="cpu")
+    return [m.prefill_paged({0: torch.arange(5), 1: torch.arange(20)}, c), m.decode_step_paged(torch.tensor([3, 4]), c)]
+
+
+def test_hooked_and_wrapped_layers_take_part_in_serving(plain_operators):
+    """As in the forward pass: a hook runs once a layer and pass and may change the output; a module in the place of a layer or its attention is called."""
+    m = _model()
+    want, seen = _serve(m), []
+    parts = [m.model.layers[0], m.model.layers[1].self_attn]
+    hooks = [p.register_forward_hook(lambda mod, a, out: seen.append(mod)) for p in parts]
+    assert all(torch.equal(a, b) for a, b in zip(_serve(m), want)) and seen == 2 * parts
+    for h in hooks:
+        h.remove()
+    hook = m.model.layers[1].self_attn.register_forward_hook(lambda mod, a, out: out * 0)
+    assert not any(torch.equal(a, b) for a, b in zip(_serve(m), want))
+    hook.remove()
+    m.model.layers[0], m.model.layers[1].self_attn = _Wrapped(m.model.layers[0]), _Wrapped(m.model.layers[1].self_attn)
+    assert all(torch.equal(a, b) for a, b in zip(_serve(m), want))
