@@ -7,6 +7,7 @@ lengths share a pool of pages; lengths and page numbers live on the device, so t
     pages = KVPages.empty(num_pages, n_kv, page_size, head_dim, device)      # one layer
     q, k_rot = paged_append(pages, k, v, cos, sin, lengths, table, q=q, cu_seqlens=cu, rotated_keys=True)   # prompts
     o = prompt_attention(q, k_rot, v, cu)
+    lengths += cu[1:] - cu[:-1]
     q, _ = paged_append(pages, k, v, cos, sin, lengths, table, q=q)          # one token a sequence
     o = paged_attention(q, pages, lengths + 1, table)
 

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import serving_ref as ref
-from tests.test_serving_gpu import _close, _packed, _pool, _prompt_reference, _starts
+from tests.test_serving_gpu import DECODE, _close, _fill, _packed, _pool, _prompt_reference, _starts
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -212,3 +212,23 @@ def test_outputs_that_lie_over_inputs():
         t.view(torch.uint8).copy_(torch.randn(t.shape).to(torch.float8_e4m3fn).view(torch.uint8))
     want = fm.paged_attention(q1, *args)
     assert torch.equal(fm.paged_attention(q1, *args, out=q1), want)
+
+
+def test_the_example_in_the_readme():
+    """Its serving lines, run as they stand: the step's output is attention over the prompt and the new token."""
+    import os
+
+    import flashmhf_b200 as fm
+    from tests.test_serving_gpu import _decode_reference
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")) as f:
+        lines = f.read().split("import flashmhf_b200 as fm\n", 1)[1].split("```", 1)[0].splitlines()
+    at = [i for i, line in enumerate(lines) if "KVPages" in line or "install_reference_seam" in line]
+    n, n_kv, page_size, head_dim, num_pages = [20, 47], 2, 16, 64, 9
+    cos, sin = ref.tables(64, head_dim)
+    x, y = _packed(sum(n), 8, head_dim, 1).cuda(), _packed(2, 8, head_dim, 2).cuda()
+    rows = [[4, 0, 7, 8], [2, 1, 3, 5]]
+    names = dict(fm=fm, num_pages=num_pages, n_kv=n_kv, page_size=page_size, head_dim=head_dim, cos=cos, sin=sin, q=x[:, :4], k=x[:, 4:6], v=x[:, 6:],
+                 q1=y[:, :4], k1=y[:, 4:6], v1=y[:, 6:], lengths=ref.ints([0, 0]), table=ref.ints(rows), cu=ref.ints(_starts(n)))
+    exec("\n".join(lines[at[0]:at[1]]), names)
+    want, _, room = _decode_reference(names["q"].cpu()[:, None], names["pages"], [21, 48], rows, head_dim ** -0.5)
+    _close(names["o"][:, None], want, room)
