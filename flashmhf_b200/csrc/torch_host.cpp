@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <optional>
 #include <vector>
 
@@ -835,22 +836,34 @@ void written(std::initializer_list<const Tensor *> ts) {
     for (const Tensor *t : ts)
         if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
-// Elements from the first to behind the last one of the dimensions from `from` on (of a tensor with elements).
-int64_t extent(const Tensor &t, int64_t from) {
-    int64_t n = 1;
-    for (int64_t i = from; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-    return n;
+// Do two bf16 tensors of the same number of dimensions share memory, b's first element lying `d` elements behind a's?  Exact for views of one buffer,
+// whose strides are the same; where strides differ, tensors whose ranges meet count as sharing.  `dims`: dimensions from the outermost stride inwards.
+bool share(const Tensor &a, const Tensor &b, const std::vector<int64_t> &dims, size_t at, int64_t d) {
+    auto extent = [&](const Tensor &t) {
+        int64_t n = 1;
+        for (size_t j = at; j < dims.size(); ++j) n += (t.size(dims[j]) - 1) * t.stride(dims[j]);
+        return n;
+    };
+    if (d >= extent(a) || -d >= extent(b)) return false;
+    if (at == dims.size()) return true;
+    const int64_t i = dims[at], na = a.size(i), nb = b.size(i), s = na > 1 ? a.stride(i) : b.stride(i);
+    if (na == 1 && nb == 1) return share(a, b, dims, at + 1, d);
+    if (na > 1 && nb > 1 && a.stride(i) != b.stride(i)) return true;
+    // Index differences x for which what the inner dimensions span can meet (two at most where no dimension steps into another's span).
+    ++at;
+    const int64_t first = std::max(-(nb - 1), (d - extent(a)) / s - 1), last = std::min(na - 1, (d + extent(b)) / s + 1);
+    if (last - first > 8) return true;
+    for (int64_t x = first; x <= last; ++x)
+        if (share(a, b, dims, at, d - x * s)) return true;
+    return false;
 }
-// Do two bf16 tensors share memory?  Exact for views of one projection (the same outermost stride, a row of either shorter than it); other tensors
-// whose ranges meet count as sharing.
 bool share(const Tensor &a, const Tensor &b) {
     if (a.numel() == 0 || b.numel() == 0) return false;
-    const int64_t d = (reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr())) / 2;
-    if (d >= extent(a, 0) || -d >= extent(b, 0)) return false;
-    const int64_t s = a.stride(0), ea = extent(a, 1), eb = extent(b, 1);
-    if (a.size(0) < 2 || b.size(0) < 2 || s != b.stride(0) || ea > s || eb > s) return true;
-    const int64_t at = ((d % s) + s) % s;
-    return at < ea || at + eb > s;
+    std::vector<int64_t> dims(a.dim());
+    std::iota(dims.begin(), dims.end(), 0);
+    auto step = [&](int64_t i) { return std::max(a.size(i) > 1 ? a.stride(i) : 0, b.size(i) > 1 ? b.stride(i) : 0); };
+    std::stable_sort(dims.begin(), dims.end(), [&](int64_t i, int64_t j) { return step(i) > step(j); });
+    return share(a, b, dims, 0, (reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr())) / 2);
 }
 // No element twice: each dimension steps over all of those with smaller strides.
 bool distinct(const Tensor &t) {

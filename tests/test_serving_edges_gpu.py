@@ -205,7 +205,23 @@ def test_outputs_that_lie_over_inputs():
         with pytest.raises(ValueError):
             fm.prompt_attention(*parts(x), cu, out=bad)
     assert torch.equal(k, parts(qkv)[1]) and torch.equal(v, parts(qkv)[2])
+    one = qkv.clone()                       # one query row inside the range of the keys, heads first, several new tokens: views that do not meet
+    row, some = parts(one)[0][30:31], ref.ints([0, 1])
+    want = fm.prompt_attention(row.clone(), k, v, some, ref.ints([0, 150]))
+    assert torch.equal(fm.prompt_attention(row, *parts(one)[1:], some, ref.ints([0, 150]), out=row), want)
+    first = qkv.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(fm.prompt_attention(*parts(first), cu, out=parts(first)[0]), fm.prompt_attention(*parts(qkv), cu))
+    with pytest.raises(ValueError):
+        fm.prompt_attention(*parts(first), cu, out=parts(first)[1])
     pages = _pool(4, 2, 32, 64, 0)
+    both = _packed(2 * 3, 8, 64, 8).cuda().view(2, 3, 8, 64)
+    where = ref.ints([40, 50]), ref.ints([[0, 1], [2, 3]])
+    for t in pages[:2]:
+        t.view(torch.uint8).copy_(torch.randn(t.shape).to(torch.float8_e4m3fn).view(torch.uint8))
+    want = fm.paged_attention(both[:, :, :4].clone(), pages, *where)
+    assert torch.equal(fm.paged_attention(both[:, :, :4], pages, *where, out=both[:, :, 4:]), want) and torch.equal(both[:, :, 4:], want)
+    with pytest.raises(ValueError):
+        fm.paged_attention(both[:, :, :4], pages, *where, out=both[:, :, 1:5])
     q1 = q[:2].clone()
     args = (pages, ref.ints([30, 50]), ref.ints([[0, 1], [2, 3]]))
     for t in pages[:2]:
