@@ -1,5 +1,6 @@
 // C-ABI layer: argument validation, dispatch to the kernel families, status word, error text.
 #include <atomic>
+#include <cstddef>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -10,8 +11,12 @@
 namespace fmhf {
 
 // Per device: the status word (first failure wins), the same for indices out of range, and the sequence number of the launch that failed.
-static __device__ int g_status_word, g_index_word;
-static __device__ unsigned g_abort_seq;
+struct DeviceWords {
+    int status;
+    unsigned abort_seq;
+    int index;
+};
+static __device__ DeviceWords g_words;
 
 namespace {
 std::atomic<uint64_t> g_launches{0};
@@ -59,19 +64,18 @@ const DeviceCtl *device_ctl() {
     if (g_ctl_ready[dev].load(std::memory_order_acquire)) return &g_ctl[dev];
     std::lock_guard<std::mutex> lk(g_mu);
     if (!g_ctl_ready[dev].load(std::memory_order_relaxed)) {
-        void *ps = nullptr, *pi = nullptr, *pa = nullptr;
+        void *words = nullptr;
         int sms = 0;
-        e = cudaGetSymbolAddress(&ps, g_status_word);
-        if (e == cudaSuccess) e = cudaGetSymbolAddress(&pi, g_index_word);
-        if (e == cudaSuccess) e = cudaGetSymbolAddress(&pa, g_abort_seq);
+        e = cudaGetSymbolAddress(&words, g_words);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess || sms < 1) {
             set_cuda_error(e, "device set-up (status word, SM count)");
             return nullptr;
         }
-        g_ctl[dev].status = static_cast<int *>(ps);
-        g_ctl[dev].index = static_cast<int *>(pi);
-        g_ctl[dev].abort_seq = static_cast<unsigned *>(pa);
+        DeviceWords *w = static_cast<DeviceWords *>(words);
+        g_ctl[dev].status = &w->status;
+        g_ctl[dev].abort_seq = &w->abort_seq;
+        g_ctl[dev].index = &w->index;
         g_ctl[dev].num_sms = sms;
         g_ctl[dev].device = dev;
         g_ctl_ready[dev].store(true, std::memory_order_release);
@@ -574,25 +578,22 @@ int flashmhf_device_status(int *code) {
     if (code) *code = 0;
     const DeviceCtl *ctl = device_ctl();
     if (!ctl) return FLASHMHF_ERR_CUDA;
+    DeviceWords *words = reinterpret_cast<DeviceWords *>(ctl->status);
     cudaError_t e = cudaDeviceSynchronize();
-    // A call reports one word and clears that one: a wait that ran out first, an index out of range with the next call.
-    auto read = [&](int *word) {
-        int v = 0;
-        if (e == cudaSuccess) e = cudaMemcpy(&v, word, sizeof(int), cudaMemcpyDeviceToHost);
-        if (e == cudaSuccess && v != 0) e = cudaMemset(word, 0, sizeof(int));
-        if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(nullptr);      // (a launch on another stream may come right after this call)
-        return v;
-    };
-    // A captured launch keeps its number in every replay: the number of the one that gave up goes together with the report of it (and before it: whatever
-    // fails here, a launch that is left out has a code in the status word).
-    if (e == cudaSuccess) e = cudaMemset(ctl->abort_seq, 0, sizeof(unsigned));
-    const int timeout = read(ctl->status), index = timeout ? 0 : read(ctl->index);
+    // A call reports one of the two and clears it: a wait that ran out first, an index out of range with the next call.  A captured launch keeps its number
+    // in every replay: the number of the one that gave up goes together with the report of it.
+    DeviceWords now{};
+    if (e == cudaSuccess) e = cudaMemcpy(&now, words, sizeof(now), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && (now.status | now.index) != 0) {
+        e = now.status ? cudaMemset(words, 0, offsetof(DeviceWords, index)) : cudaMemset(&words->index, 0, sizeof(int));
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);      // (a launch on another stream may come right after this call)
+    }
     if (e != cudaSuccess) {
         set_cuda_error(e, "flashmhf_device_status");
         return FLASHMHF_ERR_CUDA;
     }
-    if (code) *code = timeout ? timeout : index;
-    return timeout ? FLASHMHF_ERR_DEVICE_TIMEOUT : index ? FLASHMHF_ERR_DEVICE_INDEX : FLASHMHF_OK;
+    if (code) *code = now.status ? now.status : now.index;
+    return now.status ? FLASHMHF_ERR_DEVICE_TIMEOUT : now.index ? FLASHMHF_ERR_DEVICE_INDEX : FLASHMHF_OK;
 }
 
 }  // extern "C"
