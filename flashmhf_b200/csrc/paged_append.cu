@@ -3,8 +3,8 @@
 // One launch does all of it: its blocks are split between "pages" (one page, key/value head and K or V each: the scale of a page
 // depends on all of its new rows, so one block sees them all; of single tokens sixteen to a block) and "queries".  A page's new rows stay in registers between the
 // maximum and the rounding, so everything is read once and written once.  Bound: single tokens by latency (one launch: 128 sequences take as long
-// as one); prompts by HBM with heads of 128 (eight of 4096 tokens, 807 MB: 144 us = 5.6 TB/s), and by instructions and the chain of loads before
-// the first row with heads of 64, whose pages are a block's work of 8 KB (74 MB in pieces: 24 us = 3.1 TB/s; blocks that went through
+// as one); prompts by HBM with heads of 128 (eight of 4096 tokens, 807 MB: 144 to 148 us = 5.5 TB/s), and by the chain of loads before
+// the first row with heads of 64, whose pages are a block's work of 8 KB (74 MB in pieces: 24.6 us = 3.0 TB/s at 56 % of the issue slots; blocks that went through
 // several heads, asking for the next one's rows ahead, took 31 and 246 us: too many registers).
 #include <type_traits>
 

@@ -1,14 +1,15 @@
 // Attention of the newest tokens of each sequence over its pages of the 8-bit cache.
 //
-// Every code is read once and used by up to eight query rows (the query heads of a key/value head, times the new tokens), so the call
+// A code that is read is used by up to eight query rows (the query heads of a key/value head, times the new tokens), so the call
 // is bound by HBM as soon as the cache is larger than a few MB; below that by the chain of dependent loads (lengths, page numbers,
-// scales, codes) and its two launches.
+// scales, codes) and its two launches.  More than eight rows a key/value head read the cache once for each eight of them: 64 sequences of 8192, 32 / 8 heads
+// of 128, take 176 us with one new token, 187 with two, 345 with four and 655 with eight.
 //
 // Splitting.  The tokens of all (sequence, key/value head, eight query rows) are laid end to end in units of 64 and dealt out to all warps of the
 // GPU in equal contiguous runs, by lengths that only the device knows: one long sequence and a hundred short ones load the machine alike.
-// A warp works alone: its codes come by bulk copies into a ring of its own in shared memory (16 KB a warp, 192 KB on an SM: what 6.5 TB/s at
-// over a microsecond's latency take), and go from there into fragments, 32 tokens at a time: two chains of products, one look at the
-// maximum.  64 sequences of 8192 tokens, 8 heads of 128 (1.07 GB): 185 us = 5.8 TB/s; 64 of 4096, 32 heads of 64: 176 us; two of 65537, 4 heads of
+// A warp works alone: its codes come by bulk copies into a ring of its own in shared memory (16 KB a warp, 192 KB on an SM, or 18 and 216
+// with heads of 96: what 6.5 TB/s at over a microsecond's latency take), and go from there into fragments, 32 tokens at a time: two chains of products, one look at the
+// maximum.  64 sequences of 8192 tokens, 8 heads of 128 (1.07 GB): 176 to 187 us from GPU to GPU = 5.7 to 6.1 TB/s; 64 of 4096, 32 heads of 64: 176 us; two of 65537, 4 heads of
 // 128: 39 us.  In registers, 16 tokens ahead: 224, -, 61.  Sixteen warps with 12 KB and 16 tokens at a time: 179, 203, 43; eight with 24 KB: 188,
 // 204, 38, and 25 instead of 21 us for 32 ragged sequences.  Copies that run on into the next segment of a run: 187, 213, 45 (more instructions a stage
 // than the waits that they save).
@@ -46,7 +47,7 @@ struct Ring {
 // Where the scales of the pages that a run knows (32 to 64 ahead) are more than 2^8 apart, P of the smaller ones would lose its bits to the larger ones'
 // m, though other dimensions may hold nothing but theirs.  There the weights of 16 tokens have an m of their own, which puts their largest between 2^6 and
 // 2^7; what it differs from the run's multiplies their product in fp32, as the rest of a scale does that is not a power of two or beyond
-// 2^+-45.  Either way a weight is off by 2^-11 of itself, or by 2^-24 of the row's largest.
+// 2^+-45: 64 sequences of 8192 tokens, every other page 2^16 larger, 242 us instead of 176.  Either way a weight is off by 2^-11 of itself, or by 2^-24 of the row's largest.
 constexpr float kTop = 7.f, kLazyMax = 15.f;
 constexpr int kMaxExp = 45, kFar = 8;
 

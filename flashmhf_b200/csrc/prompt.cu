@@ -9,7 +9,7 @@
 // exponentials of a step and the two products 620 (a head of 64) to 1030 clk (128), but from S to P a step takes a warp some 3500 clk: tensor memory
 // both ways, the maximum, barriers, and exponentials which a warp alone asks for at 68 % of the units' rate.  So two warpgroups take the
 // steps in turn, with S and P in two buffers each.  Measured: 1770 (64) and 2000 clk (128) a step, special function units 53 % busy, tensor pipe 26
-// and 50 %; 8192 causal tokens of 32 heads of 128 at 1.16 PFLOP/s (474 us), 1.0 in a loop at the power limit.  What did not help: two tiles
+// and 50 %; 8192 causal tokens of 32 heads of 128 at 1.16 PFLOP/s (474 us) in a short loop, 0.97 to 1.0 (545 to 565 us) in a long one at the power limit.  What did not help: two tiles
 // of rows a block (half the keys from L2, but tensor memory then has P only over S, and S waits for the product that reads P: 522 against 475 us with
 // two warpgroups a tile), three warpgroups (the same reason: 547), four with 64 keys (a step costs each issuing thread 1000 clk whatever
 // its size: 581), a cubic on the FMA pipe for a quarter of the exponentials (the same time), items in the order of their length and handed out one

@@ -12,7 +12,8 @@ lengths share a pool of pages; lengths and page numbers live on the device, so t
     o = paged_attention(q, pages, lengths + 1, table)
 
 All of them are for serving: bf16 CUDA tensors, no gradients (NotImplementedError for a tensor that wants one).  What only the
-device knows, such as a page number that the pool does not have, is left out there and reported by ``check_device_status()``."""
+device knows, such as a page number that the pool does not have, is left out there and reported by ``check_device_status()``.
+What a call writes in place (pages, scales, ``out``) has a new version for autograd."""
 from typing import NamedTuple
 
 import torch
@@ -66,9 +67,11 @@ def paged_attention(q, pages, lengths, page_table, scale=None, out=None, return_
     q [B, n_q, head_dim] (one token a sequence) or [B, n_new, n_q, head_dim] with n_new up to 16, rotated and already appended;
     ``lengths`` int32 [B]: positions in the cache, those of the new tokens included (new token i sees the first
     lengths - (n_new - 1 - i)); n_q a multiple of n_kv.  ``scale`` defaults to head_dim ** -0.5.  A row that sees nothing gives
-    zeros.  ``out``: like q, its last dimension contiguous and the others in steps of 16 bytes; it may be q itself.  ``return_lse``: also the natural logarithm of the sum of exponentials, fp32, q's shape without the last dimension
+    zeros.  ``scale`` and its product with log2(e) are finite in fp32.  ``out``: like q, its last dimension contiguous and the others in steps of 16 bytes; it may be q itself.  ``return_lse``: also the natural logarithm of the sum of exponentials, fp32, q's shape without the last dimension
     (-inf for a row that sees nothing): what parts of a longer attention are merged with.  Rows of a page behind a sequence's length are
-    never used, whatever they hold; a value of a later new token that is not a finite number also reaches the new tokens before it."""
+    never used, whatever they hold; a value of a later new token that is not a finite number also reaches the new tokens before it.
+    Maxima, sums and outputs are held in fp32; a weight is rounded to fp16 before it meets the values (by 2^-11 of itself, or 2^-24 of the row's
+    largest), and a query by 2^-39 of its row's largest.  The cache is read once for each eight query rows of a key/value head."""
     o, lse = _lib.native().paged_attention(q, pages.k, pages.v, pages.k_scale, pages.v_scale, lengths, page_table, scale, out, return_lse)
     return (o, lse) if return_lse else o
 
@@ -81,6 +84,7 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     sees nothing gives zeros.  Rows of no sequence are left as they are (in a new output: undefined).  ``out`` as for ``paged_attention``; it must
     not lie over k or v.  ``return_lse`` as for
     ``paged_attention``, [T, n_q].  Sequences do not touch each other, whatever their neighbours hold; within a sequence the mask gives
-    weights of zero, so that a value which is not a finite number also reaches up to 127 rows before its own."""
+    weights of zero, so that a value which is not a finite number also reaches up to 127 rows before its own.  Maxima, sums and outputs are held in
+    fp32; a weight is rounded to bf16 before it meets the values (by 2^-8 of itself at most), the sum of weights is of unrounded ones."""
     o, lse = _lib.native().prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, out, return_lse)
     return (o, lse) if return_lse else o

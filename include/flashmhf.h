@@ -314,7 +314,8 @@ int flashmhf_paged_append(const flashmhf_paged_append_params *p, void *stream);
 
 /* o[b,i,h] = sum_p softmax_p(scale q[b,i,h].k[p]) v[p] over the first lengths[b] - (n_new-1-i) positions of the pages, for the n_new
  * newest tokens of each sequence (they are in the pages already); query head h reads key/value head h / (n_q / n_kv).  A row that sees
- * nothing gives zeros (and -inf).  q, o bf16 [B][n_new][n_q][head_dim]; lse, if not NULL, fp32 [B][n_new][n_q] contiguous: the natural
+ * nothing gives zeros (and -inf).  Weights are rounded to fp16 before they meet the values (by 2^-11 of themselves, or 2^-24 of the row's largest); sums are
+ * fp32.  The cache is read once for each eight query rows of a key/value head.  o may be q.  q, o bf16 [B][n_new][n_q][head_dim]; lse, if not NULL, fp32 [B][n_new][n_q] contiguous: the natural
  * logarithm of the sum of exponentials.  Workspace: 256-byte aligned, contents undefined before and after; two calls that may run at
  * the same time need one each.  Deterministic. */
 typedef struct flashmhf_paged_attention_params {
@@ -334,7 +335,8 @@ int flashmhf_paged_attention(const flashmhf_paged_attention_params *p, void *str
 
 /* Attention over packed sequences: rows cu_q[b] .. cu_q[b+1]-1 of q attend to rows cu_k[b] .. cu_k[b+1]-1 of k and v; causal: row r of
  * the lq rows sees key c of the lk keys where c <= r + lk - lq.  A row that sees nothing gives zeros (and -inf); rows of no sequence
- * are left as they are.  lse, if not NULL, fp32 [tokens_q][n_q] contiguous.  What the causal mask hides has a weight of zero: a value that is
+ * are left as they are.  o may be q; it must not lie over k or v.  Weights are rounded to bf16 before they meet the values, sums are fp32.
+ * lse, if not NULL, fp32 [tokens_q][n_q] contiguous.  What the causal mask hides has a weight of zero: a value that is
  * not a finite number still reaches up to 127 rows before its own, of the same sequence. */
 typedef struct flashmhf_prompt_attention_params {
     const void *q, *k, *v;            /* bf16 [tokens_q | tokens_k][n_q | n_kv][head_dim], innermost contiguous, 16-byte aligned */
